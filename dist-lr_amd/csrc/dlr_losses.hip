@@ -1,0 +1,625 @@
+// dlr_losses.hip -- softmax losses on gfx950: log-probabilities of given
+// classes and their gradient, the paired logistic (preference) loss, the
+// clipped policy loss with a KL term, and log-probabilities straight from
+// hidden states and the output layer's weights.
+//
+// Mathematics used throughout, for a row of logits z and a temperature tau:
+//   lse     = log sum_j exp(z_j / tau)
+//   logprob = z_y / tau - lse
+//   d logprob / d z_j = (1[j = y] - exp(z_j / tau - lse)) / tau
+// A row's statistics are its maximum m (exact: a logit) and
+// s = sum_j 2^((z_j - m) k), k = log2(e) / tau, in 32 bits; the difference
+// z_j - m is taken first because it is exact or nearly so for the terms that
+// count, where z_j k - m k would lose bits to |m|.  lse = m / tau + ln s and
+// everything after it is done once per row in 64 bits: a sequence's sum of
+// log-probabilities nearly cancels against the reference model's, and the
+// policy loss's gradient jumps at the clip's border.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "dlr_losses.h"
+
+namespace dlr {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// Rows may start at any element: 16-byte accesses at an element's alignment.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+// k of the row statistics
+__host__ __device__ inline float exp_scale(double temperature) { return (float)(1.44269504088896340736 / temperature); }
+#define NEG_INF (-__builtin_inff())
+
+__device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 16 bytes of a row: N elements.
+template <typename T>
+struct Pack;
+template <>
+struct Pack<float> {
+    static constexpr int N = 4;
+    static __device__ float get(const u32x4 &v, int i) { return __uint_as_float(v[i]); }
+    static __device__ u32x4 put(const float *f) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(f[i]);
+        return v;
+    }
+};
+template <>
+struct Pack<__bf16> {
+    static constexpr int N = 8;
+    static __device__ float get(const u32x4 &v, int i) {
+        const uint32_t w = v[i >> 1];
+        return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
+    }
+    static __device__ u32x4 put(const float *f) {
+        union {
+            __bf16 h[8];
+            u32x4 v;
+        } u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u.h[i] = (__bf16)f[i];  // round to nearest even
+        return u.v;
+    }
+};
+template <>
+struct Pack<_Float16> {
+    static constexpr int N = 8;
+    static __device__ float get(const u32x4 &v, int i) {
+        union {
+            u32x4 v;
+            _Float16 h[8];
+        } u;
+        u.v = v;
+        return (float)u.h[i];
+    }
+    static __device__ u32x4 put(const float *f) {
+        union {
+            _Float16 h[8];
+            u32x4 v;
+        } u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u.h[i] = (_Float16)f[i];
+        return u.v;
+    }
+};
+
+__device__ inline int64_t load_target(const void *target, int bits, int64_t t) {
+    return bits == 64 ? static_cast<const int64_t *>(target)[t] : static_cast<const int32_t *>(target)[t];
+}
+
+// ------------------------------------------------------------ row statistics
+
+struct RowStat {
+    float m;  // maximum (-inf: nothing yet)
+    float s;  // sum of 2^((z - m) k)
+};
+
+// Joins b into a.  A side that is empty (m = -inf, s = 0) adds nothing; NaN
+// and +inf anywhere make s NaN.
+__device__ inline RowStat join(RowStat a, RowStat b, float k) {
+    const float m = fmaxf(a.m, b.m);
+    const float r = m == NEG_INF ? 0.f : m;
+    return {m, a.s * exp2_hw((a.m - r) * k) + b.s * exp2_hw((b.m - r) * k)};
+}
+
+__device__ inline RowStat join_wave(RowStat a, float k) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        RowStat b{__shfl_xor(a.m, o), __shfl_xor(a.s, o)};
+        a = join(a, b, k);
+    }
+    return a;
+}
+
+// The block's statistic, in every thread.
+template <int NT>
+__device__ inline RowStat join_block(RowStat a, float k, RowStat *lds) {
+    a = join_wave(a, k);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) lds[wave] = a;
+    __syncthreads();
+    RowStat r = lds[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) r = join(r, lds[w], k);
+    return r;
+}
+
+// One pass over a row: U packs a thread in flight, one rescaling of the
+// running sum per U packs.
+template <typename T, int NT, int U>
+__device__ inline RowStat row_stat(const T *row, int vocab, float k) {
+    using PK = Pack<T>;
+    constexpr int N = PK::N;
+    const int packs = vocab / N;
+    RowStat a{NEG_INF, 0.f};
+    for (int base = threadIdx.x; base < packs; base += NT * U) {
+        u32x4 v[U];
+        bool have[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = base + u * NT;
+            have[u] = p < packs;
+            if (have[u]) v[u] = *reinterpret_cast<const u32x4_any *>(row + (int64_t)p * N);
+        }
+        float m = a.m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (have[u]) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) m = fmaxf(m, PK::get(v[u], i));
+            }
+        const float r = m == NEG_INF ? 0.f : m;
+        float s = a.s * exp2_hw((a.m - r) * k);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (have[u]) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) s += exp2_hw((PK::get(v[u], i) - r) * k);
+            }
+        a.m = m;
+        a.s = s;
+    }
+    const int tail = packs * N + threadIdx.x;
+    if (tail < vocab) {
+        const float z = (float)row[tail];
+        a = join(a, RowStat{z, z == z ? 1.f : z}, k);
+    }
+    return a;
+}
+
+// The difference to the maximum first: lse itself cannot hold ln s where the
+// logits are huge (a row masked with the type's lowest value).
+__device__ inline double target_logprob(float zy, float m, double ln_s, double tau) {
+    return ((double)zy - (double)m) / tau - ln_s;
+}
+
+// ----------------------------------------------------- token log-probabilities
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t stride, int vocab, const void *target,
+                                                      int target_bits, float k, double tau, float *logprob, float *lse) {
+    __shared__ RowStat lds[NT / 64];
+    const int64_t t = blockIdx.x;
+    const int64_t y = load_target(target, target_bits, t);
+    if (y < 0) {  // ignored: the row is not read
+        if (threadIdx.x == 0) {
+            logprob[t] = 0.f;
+            lse[t] = 0.f;
+        }
+        return;
+    }
+    const T *row = logits + t * stride;
+    const float zy = y < vocab ? (float)row[y] : __builtin_nanf("");
+    const RowStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
+    if (threadIdx.x == 0) {
+        const double ln = log((double)a.s);
+        lse[t] = (float)(a.m / tau + ln);
+        logprob[t] = (float)target_logprob(zy, a.m, ln, tau);
+    }
+}
+
+// Writes `out`'s row of zeros.
+template <typename T, int NT>
+__device__ inline void zero_row(T *out, int vocab) {
+    constexpr int N = Pack<T>::N;
+    const int packs = vocab / N;
+    const u32x4 z = {0u, 0u, 0u, 0u};
+    for (int p = threadIdx.x; p < packs; p += NT) *reinterpret_cast<u32x4_any *>(out + (int64_t)p * N) = z;
+    const int tail = packs * N + threadIdx.x;
+    if (tail < vocab) out[tail] = (T)0.f;
+}
+
+// out_j = (j = y ? c : 0) + neg * 2^(z_j a + b): the softmax residual, the
+// exponent's two forms chosen by the caller (see the kernels).  Each thread
+// reads a pack before it writes it, so out may be the row itself.
+template <typename T, int NT, int U, typename F>
+__device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, float c, F prob) {
+    using PK = Pack<T>;
+    constexpr int N = PK::N;
+    const int packs = vocab / N;
+    for (int base = threadIdx.x; base < packs; base += NT * U) {
+        u32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = base + u * NT;
+            if (p < packs) v[u] = *reinterpret_cast<const u32x4_any *>(row + (int64_t)p * N);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = base + u * NT;
+            if (p >= packs) continue;
+            float f[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = prob(PK::get(v[u], i));
+            const int64_t at = y - (int64_t)p * N;
+            if (at >= 0 && at < N) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) f[i] += i == at ? c : 0.f;
+            }
+            *reinterpret_cast<u32x4_any *>(out + (int64_t)p * N) = PK::put(f);
+        }
+    }
+    const int tail = packs * N + threadIdx.x;
+    if (tail < vocab) out[tail] = (T)(prob((float)row[tail]) + (tail == y ? c : 0.f));
+}
+
+// 32 bits of lse are a relative error of |lse| 2^-24 in every probability:
+// below 1e-5 up to here.  Rows beyond (logits in the hundreds, rows masked
+// with the type's lowest value) take their statistics again.
+constexpr float kLseExact = 128.f;
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int64_t stride, int vocab,
+                                                           const void *target, int target_bits, double tau,
+                                                           const float *lse, const float *grad, T *out,
+                                                           int64_t out_stride) {
+    const int64_t t = blockIdx.x;
+    const int64_t y = load_target(target, target_bits, t);
+    T *o = out + t * out_stride;
+    const float g = y < 0 ? 0.f : grad[t];
+    if (g == 0.f) {  // ignored, or nothing flows back: the row is not read
+        zero_row<T, NT>(o, vocab);
+        return;
+    }
+    const float c = y < vocab ? (float)(g / tau) : __builtin_nanf("");
+    const float l = lse[t];
+    if (fabsf(l) > kLseExact) {
+        __shared__ RowStat lds[NT / 64];
+        const float k = exp_scale(tau);
+        const RowStat a = join_block<NT>(row_stat<T, NT, 4>(logits + t * stride, vocab, k), k, lds);
+        const float neg = -c / a.s, m = a.m;
+        residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
+                               [=](float z) { return neg * exp2_hw((z - m) * k); });
+        return;
+    }
+    const float it = (float)(1.0 / tau);
+    residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
+                           [=](float z) { return -c * exp2_hw(__builtin_fmaf(z, it, -l) * kLog2e); });
+}
+
+// ---------------------------------------------------------------- policy loss
+
+struct PolicyOut {
+    float *loss, *logprob, *kl;
+    uint8_t *clipped;
+};
+
+// One row's loss from its log-probability, in 64 bits.  Returns d loss /
+// d logprob times the weight.
+__device__ inline double policy_token(double lp, const dlr_policy &p, int64_t t, double w, const PolicyOut &o) {
+    const double adv = p.advantage[t];
+    const double ratio = exp(lp - (double)p.old_logprob[t]);
+    const double lo = 1.0 - p.clip_low, hi = 1.0 + p.clip_high;
+    // min(ratio A, clip(ratio) A): the clip holds back gains above hi and
+    // losses below lo; A = 0 has no surrogate (0 * inf otherwise)
+    const bool held = (adv > 0.0 && ratio > hi) || (adv < 0.0 && ratio < lo);
+    const double surrogate = adv == 0.0 ? 0.0 : (held ? (adv > 0.0 ? hi : lo) : ratio) * adv;
+    double kl = 0.0, slope = held || adv == 0.0 ? 0.0 : -ratio * adv;
+    double loss = -surrogate;
+    if (p.ref_logprob) {
+        const double gap = (double)p.ref_logprob[t] - lp;
+        const double e = expm1(gap);
+        kl = e - gap;
+        if (p.kl_coef != 0.0) {
+            loss += p.kl_coef * kl;
+            slope -= p.kl_coef * e;
+        }
+    }
+    if (ratio != ratio) loss = slope = ratio;  // NaN log-probabilities stay visible
+    o.loss[t] = (float)loss;
+    o.logprob[t] = (float)lp;
+    o.kl[t] = (float)kl;
+    o.clipped[t] = held;
+    return slope * w;
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t stride, int vocab, const void *target,
+                                                    int target_bits, float k, double tau, dlr_policy p, PolicyOut po,
+                                                    T *out, int64_t out_stride) {
+    __shared__ RowStat lds[NT / 64];
+    __shared__ float coef;
+    const int64_t t = blockIdx.x;
+    const int64_t y = load_target(target, target_bits, t);
+    const float w = p.weight ? p.weight[t] : 1.f;
+    if (y < 0 || w == 0.f) {
+        if (threadIdx.x == 0) {
+            po.loss[t] = po.logprob[t] = po.kl[t] = 0.f;
+            po.clipped[t] = 0;
+        }
+        if (out) zero_row<T, NT>(out + t * out_stride, vocab);
+        return;
+    }
+    const T *row = logits + t * stride;
+    const float zy = y < vocab ? (float)row[y] : __builtin_nanf("");
+    const RowStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
+    if (threadIdx.x == 0) {
+        const double lp = target_logprob(zy, a.m, log((double)a.s), tau);
+        coef = (float)(policy_token(lp, p, t, w, po) / tau);
+    }
+    if (!out) return;
+    __syncthreads();
+    const float c = coef, neg = -c / a.s, m = a.m;
+    residual_row<T, NT, 4>(row, out + t * out_stride, vocab, y, c,
+                           [=](float z) { return neg * exp2_hw((z - m) * k); });
+}
+
+// ------------------------------------------------------------ preference loss
+
+__device__ inline double sum_block(double v, double *lds) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double r = 0.0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) r += lds[w];
+    return r;
+}
+
+struct PairOut {
+    float *loss, *chosen, *rejected, *grad;
+};
+
+// softplus(-u) = -log sigma(u), without overflow on either side
+__device__ inline double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+
+// One pair a block: the two sequences' sums of log ratios in 64 bits, the
+// logistic loss of their difference, and the pair's one slope written over
+// its tokens.
+template <int NT>
+__global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOut o) {
+    __shared__ double lds[NT / 64];
+    const int64_t P = p.pairs, T = p.tokens;
+    if (o.grad && blockIdx.x == 0) {  // tokens of no sequence: before the first, behind the last
+        int64_t b = P ? p.offsets[0] : T, e = P ? p.offsets[2 * P] : T;
+        b = b < 0 ? 0 : b > T ? T : b;
+        e = e < b ? b : e > T ? T : e;
+        for (int64_t i = threadIdx.x; i < b; i += NT) o.grad[i] = 0.f;
+        for (int64_t i = e + threadIdx.x; i < T; i += NT) o.grad[i] = 0.f;
+    }
+    if (!P) return;
+    const int64_t pair = blockIdx.x;
+    double reward[2], scale[2];
+    int64_t first[2], last[2];
+    bool bad = false;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int64_t seq = pair + q * P;
+        int64_t b = p.offsets[seq], e = p.offsets[seq + 1];
+        if (b < 0 || e < b || e > T) {  // not a range of the tokens: nothing is read or written
+            bad = true;
+            b = e = 0;
+        }
+        first[q] = b;
+        last[q] = e;
+        double sum = 0.0, count = 0.0;
+        for (int64_t i = b + threadIdx.x; i < e; i += NT)
+            if (!p.mask || p.mask[i]) {
+                sum += (double)p.logprob[i] - (p.ref_logprob ? (double)p.ref_logprob[i] : 0.0);
+                count += 1.0;
+            }
+        sum = sum_block(sum, lds);
+        scale[q] = p.beta;
+        if (p.average) {
+            count = sum_block(count, lds);
+            scale[q] /= count > 1.0 ? count : 1.0;
+        }
+        reward[q] = scale[q] * sum;
+    }
+    const double eps = p.label_smoothing;
+    double u = reward[0] - reward[1] - p.margin;
+    if (bad) u = reward[0] = reward[1] = __builtin_nan("");
+    const double w = p.weight ? (double)p.weight[pair] : 1.0;
+    if (threadIdx.x == 0) {
+        o.loss[pair] = (float)((1.0 - eps) * softplus(-u) + eps * softplus(u));
+        o.chosen[pair] = (float)reward[0];
+        o.rejected[pair] = (float)reward[1];
+    }
+    if (!o.grad) return;
+    // d loss / d u = sigma(u) - (1 - eps)
+    const double slope = w == 0.0 ? 0.0 : w * (eps / (1.0 + exp(-u)) - (1.0 - eps) / (1.0 + exp(u)));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const float g = (float)((q ? -slope : slope) * scale[q]);
+        for (int64_t i = first[q] + threadIdx.x; i < last[q]; i += NT)
+            o.grad[i] = !p.mask || p.mask[i] ? g : 0.f;
+    }
+}
+
+// -------------------------------------------------- head log-probabilities
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ inline f32x4 mfma(const u32x4 &a, const u32x4 &b, f32x4 c, __bf16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+__device__ inline f32x4 mfma(const u32x4 &a, const u32x4 &b, f32x4 c, _Float16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+// 8 elements of row `r` from element k on; what lies outside [0, rows) x
+// [0, dim) is 0 and not read.
+__device__ inline u32x4 load8(const uint16_t *base, int64_t stride, int64_t r, int64_t rows, int k, int dim) {
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (r >= rows) return v;
+    const uint16_t *s = base + r * stride + k;
+    if (k + 8 <= dim) return *reinterpret_cast<const u32x4_any *>(s);
+    union {
+        uint16_t h[8];
+        u32x4 v;
+    } u;
+    u.v = v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k + i < dim) u.h[i] = s[i];
+    return u.v;
+}
+
+constexpr int kTileV = 128, kTileT = 128, kTileK = 64, kLdsRow = kTileK + 8;
+
+// One tile of kTileV classes x kTileT tokens: logits = head . hidden^T by
+// MFMA in 32 bits, never written; per token the tile's (maximum, sum) goes
+// to part[tile][token], and the target's logit to zy[token].  Classes lie
+// along the MFMA's rows, so a token's values sit in one lane column.
+template <typename T>
+__global__ __launch_bounds__(256) void k_head_tile(dlr_head h, float2 *part, float *zy) {
+    __shared__ __attribute__((aligned(16))) uint16_t sw[kTileV * kLdsRow];
+    __shared__ __attribute__((aligned(16))) uint16_t sx[kTileT * kLdsRow];
+    __shared__ RowStat st[2][kTileT];
+    const uint16_t *head = static_cast<const uint16_t *>(h.head), *hidden = static_cast<const uint16_t *>(h.hidden);
+    const int64_t v0 = (int64_t)blockIdx.x * kTileV, t0 = (int64_t)blockIdx.y * kTileT;
+    const int dim = (int)h.dim;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wv = wave >> 1, wt = wave & 1;
+    f32x4 acc[4][4] = {};
+    for (int k0 = 0; k0 < dim; k0 += kTileK) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = tid + i * 256, r = c >> 3, kk = (c & 7) * 8;
+            *reinterpret_cast<u32x4 *>(&sw[r * kLdsRow + kk]) = load8(head, h.head_stride, v0 + r, h.vocab, k0 + kk, dim);
+            *reinterpret_cast<u32x4 *>(&sx[r * kLdsRow + kk]) =
+                load8(hidden, h.hidden_stride, t0 + r, h.rows, k0 + kk, dim);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < kTileK; kk += 32) {
+            u32x4 a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = *reinterpret_cast<u32x4 *>(&sw[(wv * 64 + i * 16 + (lane & 15)) * kLdsRow + kk + (lane >> 4) * 8]);
+                b[i] = *reinterpret_cast<u32x4 *>(&sx[(wt * 64 + i * 16 + (lane & 15)) * kLdsRow + kk + (lane >> 4) * 8]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
+        }
+    }
+    const float k = exp_scale(h.temperature);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t t = t0 + wt * 64 + j * 16 + (lane & 15);
+        const int64_t y = t < h.rows ? load_target(h.target, h.target_bits, t) : -1;
+        RowStat a{NEG_INF, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t v = v0 + wv * 64 + i * 16 + (lane >> 4) * 4 + e;
+                if (v < h.vocab) {
+                    const float z = acc[i][j][e];
+                    a = join(a, RowStat{z, z == z ? 1.f : z}, k);
+                    if (v == y) zy[t] = z;
+                }
+            }
+        a = join(a, RowStat{__shfl_xor(a.m, 16), __shfl_xor(a.s, 16)}, k);
+        a = join(a, RowStat{__shfl_xor(a.m, 32), __shfl_xor(a.s, 32)}, k);
+        if (lane < 16) st[wv][wt * 64 + j * 16 + lane] = a;
+    }
+    __syncthreads();
+    if (tid < kTileT && t0 + tid < h.rows) {
+        const RowStat a = join(st[0][tid], st[1][tid], k);
+        part[(int64_t)blockIdx.x * h.rows + t0 + tid] = make_float2(a.m, a.s);
+    }
+}
+
+// The tiles' statistics of one token, joined by one wave.
+__global__ __launch_bounds__(256) void k_head_join(dlr_head h, int64_t tiles, const float2 *part, const float *zy,
+                                                   float *logprob, float *lse) {
+    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= h.rows) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t y = load_target(h.target, h.target_bits, t);
+    const float k = exp_scale(h.temperature);
+    RowStat a{NEG_INF, 0.f};
+    if (y >= 0)
+        for (int64_t i = lane; i < tiles; i += 64) {
+            const float2 q = part[i * h.rows + t];
+            a = join(a, RowStat{q.x, q.y}, k);
+        }
+    a = join_wave(a, k);
+    if (lane) return;
+    const double tau = h.temperature;
+    const double ln = log((double)a.s);
+    lse[t] = y < 0 ? 0.f : (float)(a.m / tau + ln);
+    logprob[t] = y < 0 ? 0.f : y < h.vocab ? (float)target_logprob(zy[t], a.m, ln, tau) : __builtin_nanf("");
+}
+
+}  // namespace
+
+template <typename F>
+static hipError_t by_dtype(int dtype, F f) {
+    switch (dtype) {
+        case DLR_DTYPE_F32: f(float()); break;
+        case DLR_DTYPE_BF16: f(__bf16()); break;
+        default: f(_Float16()); break;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
+    return by_dtype(x.dtype, [&](auto e) {
+        using T = decltype(e);
+        k_token_logprob<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
+            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
+            x.temperature, logprob, lse);
+    });
+}
+
+hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad,
+                                     void *out, int64_t out_stride) {
+    return by_dtype(x.dtype, [&](auto e) {
+        using T = decltype(e);
+        k_token_logprob_grad<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
+            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, x.temperature, lse,
+            grad, static_cast<T *>(out), out_stride);
+    });
+}
+
+hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, float *loss, float *logprob,
+                              float *kl, uint8_t *clipped, void *out, int64_t out_stride) {
+    return by_dtype(x.dtype, [&](auto e) {
+        using T = decltype(e);
+        k_policy_loss<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
+            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
+            x.temperature, p, PolicyOut{loss, logprob, kl, clipped}, static_cast<T *>(out), out_stride);
+    });
+}
+
+hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float *loss, float *chosen,
+                                  float *rejected, float *grad) {
+    k_preference_loss<256>
+        <<<dim3((unsigned)(p.pairs ? p.pairs : 1)), 256, 0, st>>>(p, PairOut{loss, chosen, rejected, grad});
+    return hipGetLastError();
+}
+
+int64_t head_workspace(int64_t rows, int64_t vocab) {
+    const int64_t tiles = (vocab + kTileV - 1) / kTileV;
+    return rows * tiles * (int64_t)sizeof(float2) + rows * (int64_t)sizeof(float);
+}
+
+hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
+    const int64_t tiles = (h.vocab + kTileV - 1) / kTileV;
+    float2 *part = static_cast<float2 *>(workspace);
+    float *zy = reinterpret_cast<float *>(part + tiles * h.rows);
+    const dim3 grid((unsigned)tiles, (unsigned)((h.rows + kTileT - 1) / kTileT));
+    if (h.dtype == DLR_DTYPE_BF16)
+        k_head_tile<__bf16><<<grid, 256, 0, st>>>(h, part, zy);
+    else
+        k_head_tile<_Float16><<<grid, 256, 0, st>>>(h, part, zy);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_head_join<<<dim3((unsigned)((h.rows + 3) / 4)), 256, 0, st>>>(h, tiles, part, zy, logprob, lse);
+    return hipGetLastError();
+}
+
+}  // namespace dlr

@@ -29,6 +29,7 @@ RESIDENCY_AUTO, RESIDENCY_DEVICE, RESIDENCY_STREAM = 0, 1, 2
 STAGE_MARGIN, STAGE_GRADIENT, STAGE_UPDATE = 0, 1, 2
 TRANSPORT_NONE, TRANSPORT_RCCL, TRANSPORT_LOOPBACK = 0, 1, 2
 ORDER_REFERENCE, ORDER_FAST = 0, 1
+E_ARG = -1  # bad argument / shape mismatch
 E_DEVICE = -8  # an in-launch hand-off never came (dlr_sync)
 # test-only producer faults (dlr_set_fault)
 FAULT_NONE, FAULT_MG_PUBLISH, FAULT_REF_PUBLISH, FAULT_HOT_RING = 0, 1, 2, 3
@@ -58,6 +59,8 @@ SYMBOLS = [
     "dlr_timing", "dlr_kernel_time", "dlr_stage_time", "dlr_stage_counters", "dlr_train_layout", "dlr_train_band_rows", "dlr_train_relabeled", "dlr_train_unit_values", "dlr_train_product_margin", "dlr_train_pm_strided", "dlr_train_hot_columns", "dlr_train_row_rounds",
     "dlr_set_exchange_overlap", "dlr_exchange_overlap", "dlr_set_exchange_pieces", "dlr_exchange_pieces",
     "dlr_memory_info", "dlr_stream_bytes",
+    "dlr_token_logprob", "dlr_token_logprob_grad", "dlr_policy_loss", "dlr_preference_loss",
+    "dlr_head_logprob_workspace", "dlr_head_logprob",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -225,6 +228,12 @@ _sig("dlr_set_exchange_pieces", C.c_int, P, C.c_int)
 _sig("dlr_exchange_pieces", C.c_int, P)
 _sig("dlr_memory_info", C.c_int, P, C.POINTER(i64), C.POINTER(i64))
 _sig("dlr_stream_bytes", C.c_int, P, C.POINTER(i64), C.POINTER(i64))
+_sig("dlr_token_logprob", C.c_int, C.c_int, P, P, P, P)
+_sig("dlr_token_logprob_grad", C.c_int, C.c_int, P, P, P, P, P, i64)
+_sig("dlr_policy_loss", C.c_int, C.c_int, P, P, P, P, P, P, P, P, i64)
+_sig("dlr_preference_loss", C.c_int, C.c_int, P, P, P, P, P, P)
+_sig("dlr_head_logprob_workspace", i64, i64, i64, i64)
+_sig("dlr_head_logprob", C.c_int, C.c_int, P, P, P, i64, P, P)
 
 
 class DLRError(RuntimeError):

@@ -1,0 +1,275 @@
+"""Softmax losses on torch tensors (the device section of
+include/distlr_amd.h): log-probabilities of given classes and their gradient,
+the paired logistic (preference) loss, the clipped policy loss, and
+log-probabilities straight from hidden states and the output layer's weights.
+
+The many-class counterparts of the engine's margin, residual and log-loss
+(lr.cc:35-40, 47-63).  Like the engine they return gradients, they do not
+record an autograd graph: pass one on with ``logits.backward(grad)``.
+
+Every tensor is on one GPU.  The work runs on torch's current stream of that
+GPU and may be captured into a graph; results and scratch memory come from
+torch's allocator.  As with torch's own operators, a tensor made on another
+stream has to be waited for by the caller.  Arguments that do not fit raise
+``DLRError`` with code ``E_ARG`` before anything is enqueued.
+
+Import torch before this package, so that the process has one HIP runtime.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import E_ARG, DLRError, _check, lib
+
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+_TARGET_BITS = {torch.int32: 32, torch.int64: 64}
+
+
+def _one_runtime() -> None:
+    """A stream of one HIP runtime means nothing to another one."""
+    try:
+        with open("/proc/self/maps") as f:
+            seen = {line.split()[-1] for line in f if "/libamdhip64.so" in line}
+    except OSError:
+        return
+    if len(seen) > 1:
+        raise ImportError(f"two HIP runtimes in this process ({', '.join(sorted(seen))}): import torch before distlr_amd")
+
+
+_one_runtime()
+
+
+class _Logits(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("target", C.c_void_p), ("rows", C.c_int64), ("vocab", C.c_int64),
+                ("row_stride", C.c_int64), ("dtype", C.c_int32), ("target_bits", C.c_int32),
+                ("temperature", C.c_double)]
+
+
+class _Policy(C.Structure):
+    _fields_ = [("old_logprob", C.c_void_p), ("ref_logprob", C.c_void_p), ("advantage", C.c_void_p),
+                ("weight", C.c_void_p), ("clip_low", C.c_double), ("clip_high", C.c_double), ("kl_coef", C.c_double)]
+
+
+class _Preference(C.Structure):
+    _fields_ = [("logprob", C.c_void_p), ("ref_logprob", C.c_void_p), ("mask", C.c_void_p), ("offsets", C.c_void_p),
+                ("weight", C.c_void_p), ("pairs", C.c_int64), ("tokens", C.c_int64), ("beta", C.c_double),
+                ("label_smoothing", C.c_double), ("margin", C.c_double), ("average", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class _Head(C.Structure):
+    _fields_ = [("hidden", C.c_void_p), ("head", C.c_void_p), ("target", C.c_void_p), ("rows", C.c_int64),
+                ("vocab", C.c_int64), ("dim", C.c_int64), ("hidden_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("dtype", C.c_int32), ("target_bits", C.c_int32), ("temperature", C.c_double)]
+
+
+class PolicyLoss(NamedTuple):
+    """Per row; grad has the logits' shape and type (None if not asked for)."""
+    loss: torch.Tensor
+    logprob: torch.Tensor
+    kl: torch.Tensor
+    clipped: torch.Tensor
+    grad: Optional[torch.Tensor]
+
+
+class PreferenceLoss(NamedTuple):
+    """Per pair; grad is per token (None if not asked for)."""
+    loss: torch.Tensor
+    chosen_reward: torch.Tensor
+    rejected_reward: torch.Tensor
+    grad: Optional[torch.Tensor]
+
+
+def _refuse(why: str):
+    raise DLRError(E_ARG, why)
+
+
+def _gpu(name: str, t) -> torch.device:
+    if not isinstance(t, torch.Tensor):
+        _refuse(f"{name} must be a torch tensor")
+    if t.device.type != "cuda":
+        _refuse(f"{name} must be on a GPU (it is on {t.device})")
+    return t.device
+
+
+def _matrix(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 2:
+        _refuse(f"{name} must have 2 dimensions (it has {t.dim()})")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        _refuse(f"{name} must be contiguous within a row")
+
+
+def _vector(name: str, t, device: torch.device, dtypes, length: int) -> torch.Tensor:
+    """A 1-D tensor of one of `dtypes`; a strided one is copied."""
+    if _gpu(name, t) != device:
+        _refuse(f"{name} is on {t.device}, not on {device}")
+    if t.dtype not in dtypes:
+        _refuse(f"{name} must be {' or '.join(str(d) for d in dtypes)} (it is {t.dtype})")
+    if t.dim() != 1 or t.shape[0] != length:
+        _refuse(f"{name} must have shape ({length},) (it has {tuple(t.shape)})")
+    return t.contiguous()
+
+
+_F32 = (torch.float32,)
+_INTS = (torch.int64, torch.int32)
+_BOOL = (torch.bool,)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _logits(logits: torch.Tensor, target: torch.Tensor, temperature: float):
+    device = _gpu("logits", logits)
+    _matrix("logits", logits)
+    if logits.dtype not in _DTYPES:
+        _refuse(f"logits must be float32, bfloat16 or float16 (they are {logits.dtype})")
+    rows, vocab = logits.shape
+    target = _vector("target", target, device, _INTS, rows)
+    return device, target, _Logits(logits.data_ptr(), target.data_ptr(), rows, vocab, logits.stride(0),
+                                   _DTYPES[logits.dtype], _TARGET_BITS[target.dtype], temperature)
+
+
+def _grad_like(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if _gpu("out", out) != logits.device or out.dtype != logits.dtype or out.shape != logits.shape:
+        _refuse("out must have the logits' device, type and shape")
+    _matrix("out", out)
+    return out
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def token_logprob(logits: torch.Tensor, target: torch.Tensor, *,
+                  temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(logprob, lse), float32 per row: logprob = logits[t, target[t]] /
+    temperature - lse, lse = log sum exp(logits[t] / temperature).  A
+    negative target marks a row that takes no part: 0, not read
+    (dlr_token_logprob)."""
+    device, target, x = _logits(logits, target, temperature)
+    out = torch.empty((2, x.rows), dtype=torch.float32, device=device)
+    logprob, lse = out[0], out[1]
+    _check(lib.dlr_token_logprob(device.index, _stream(device), C.byref(x), logprob.data_ptr(), lse.data_ptr()))
+    return logprob, lse
+
+
+def token_logprob_grad(logits: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor, *,
+                       temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient with respect to the logits of sum(grad * logprob), in the
+    logits' type; lse is token_logprob's.  Rows with a negative target or
+    grad 0 are 0.  out may be the logits themselves
+    (dlr_token_logprob_grad)."""
+    device, target, x = _logits(logits, target, temperature)
+    lse = _vector("lse", lse, device, _F32, x.rows)
+    grad = _vector("grad", grad, device, _F32, x.rows)
+    out = _grad_like(logits, out)
+    _check(lib.dlr_token_logprob_grad(device.index, _stream(device), C.byref(x), lse.data_ptr(), grad.data_ptr(),
+                                      out.data_ptr(), out.stride(0)))
+    return out
+
+
+def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logprob: torch.Tensor, advantage: torch.Tensor, *,
+                ref_logprob: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
+                clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
+                grad: bool = True, out: Optional[torch.Tensor] = None) -> PolicyLoss:
+    """The clipped policy loss with a KL term, per row, and the gradient of
+    sum(weight * loss) with respect to the logits, in one pass
+    (dlr_policy_loss).
+
+    loss = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) +
+    kl_coef kl, ratio = exp(logprob - old_logprob), kl = exp(ref - logprob) -
+    (ref - logprob) - 1 (0 without ref_logprob).  weight defaults to 1: give
+    each row its share of a mean.  Rows with a negative target or weight 0
+    take no part.  clipped: where the clip holds the surrogate.  out: the
+    gradient's tensor, which may be the logits themselves."""
+    device, target, x = _logits(logits, target, temperature)
+    old_logprob = _vector("old_logprob", old_logprob, device, _F32, x.rows)
+    advantage = _vector("advantage", advantage, device, _F32, x.rows)
+    if ref_logprob is not None:
+        ref_logprob = _vector("ref_logprob", ref_logprob, device, _F32, x.rows)
+    if weight is not None:
+        weight = _vector("weight", weight, device, _F32, x.rows)
+    if out is not None and not grad:
+        _refuse("out is the gradient's tensor: grad must be True")
+    dz = _grad_like(logits, out) if grad else None
+    p = _Policy(_ptr(old_logprob), _ptr(ref_logprob), _ptr(advantage), _ptr(weight), clip_low, clip_high, kl_coef)
+    res = torch.empty((3, x.rows), dtype=torch.float32, device=device)
+    loss, logprob, kl = res[0], res[1], res[2]
+    clipped = torch.empty(x.rows, dtype=torch.bool, device=device)
+    _check(lib.dlr_policy_loss(device.index, _stream(device), C.byref(x), C.byref(p), loss.data_ptr(),
+                               logprob.data_ptr(), kl.data_ptr(), clipped.data_ptr(), _ptr(dz),
+                               0 if dz is None else dz.stride(0)))
+    return PolicyLoss(loss, logprob, kl, clipped, dz)
+
+
+def preference_loss(logprob: torch.Tensor, ref_logprob: Optional[torch.Tensor], offsets: torch.Tensor, *, beta: float,
+                    label_smoothing: float = 0.0, margin: float = 0.0, mask: Optional[torch.Tensor] = None,
+                    weight: Optional[torch.Tensor] = None, average: bool = False,
+                    grad: bool = True) -> PreferenceLoss:
+    """The paired logistic loss over packed sequences of token
+    log-probabilities, per pair, and the gradient of sum(weight * loss) with
+    respect to logprob (dlr_preference_loss).
+
+    offsets (int64, 2 P + 1 ascending): sequence i is tokens [offsets[i],
+    offsets[i + 1]); pair p compares sequence p (preferred) with P + p.
+    reward = beta * sum(logprob - ref_logprob) over the tokens with mask
+    (average: per counted token); loss = -(1 - label_smoothing) log sigma(u) -
+    label_smoothing log sigma(-u), u = chosen_reward - rejected_reward -
+    margin.  weight (P) defaults to 1."""
+    device = _gpu("logprob", logprob)
+    tokens = logprob.shape[0] if logprob.dim() == 1 else -1
+    if tokens < 0:
+        _refuse(f"logprob must have 1 dimension (it has {logprob.dim()})")
+    logprob = _vector("logprob", logprob, device, _F32, tokens)
+    if ref_logprob is not None:
+        ref_logprob = _vector("ref_logprob", ref_logprob, device, _F32, tokens)
+    if _gpu("offsets", offsets).type == "cuda" and (offsets.dim() != 1 or offsets.shape[0] % 2 != 1):
+        _refuse("offsets must have 2 P + 1 entries")
+    pairs = offsets.shape[0] // 2
+    offsets = _vector("offsets", offsets, device, (torch.int64,), 2 * pairs + 1)
+    if mask is not None:
+        mask = _vector("mask", mask, device, _BOOL, tokens)
+    if weight is not None:
+        weight = _vector("weight", weight, device, _F32, pairs)
+    p = _Preference(_ptr(logprob), _ptr(ref_logprob), _ptr(mask), _ptr(offsets), _ptr(weight), pairs, tokens, beta,
+                    label_smoothing, margin, 1 if average else 0, 0)
+    res = torch.empty((3, pairs), dtype=torch.float32, device=device)
+    loss, chosen, rejected = res[0], res[1], res[2]
+    dl = torch.empty(tokens, dtype=torch.float32, device=device) if grad else None
+    _check(lib.dlr_preference_loss(device.index, _stream(device), C.byref(p), loss.data_ptr(), chosen.data_ptr(),
+                                   rejected.data_ptr(), _ptr(dl)))
+    return PreferenceLoss(loss, chosen, rejected, dl)
+
+
+def head_logprob(hidden: torch.Tensor, head: torch.Tensor, target: torch.Tensor, *,
+                 temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """token_logprob of the logits hidden (rows x dim) . head^T (vocab x dim),
+    which are never written out: scoring by a model that is not trained.
+    bfloat16 or float16, sums in 32 bits (dlr_head_logprob)."""
+    device = _gpu("hidden", hidden)
+    _matrix("hidden", hidden)
+    if _gpu("head", head) != device:
+        _refuse(f"head is on {head.device}, not on {device}")
+    _matrix("head", head)
+    if hidden.dtype not in (torch.bfloat16, torch.float16) or head.dtype != hidden.dtype:
+        _refuse(f"hidden and head must both be bfloat16 or float16 (they are {hidden.dtype} and {head.dtype})")
+    rows, dim = hidden.shape
+    if head.shape[1] != dim:
+        _refuse(f"hidden has rows of {dim}, head of {head.shape[1]}")
+    target = _vector("target", target, device, _INTS, rows)
+    h = _Head(hidden.data_ptr(), head.data_ptr(), target.data_ptr(), rows, head.shape[0], dim, hidden.stride(0),
+              head.stride(0), _DTYPES[hidden.dtype], _TARGET_BITS[target.dtype], temperature)
+    need = _check(lib.dlr_head_logprob_workspace(rows, head.shape[0], dim))
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    out = torch.empty((2, rows), dtype=torch.float32, device=device)
+    logprob, lse = out[0], out[1]
+    _check(lib.dlr_head_logprob(device.index, _stream(device), C.byref(h), workspace.data_ptr(), need,
+                                logprob.data_ptr(), lse.data_ptr()))
+    return logprob, lse
