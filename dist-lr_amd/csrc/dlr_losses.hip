@@ -28,12 +28,27 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLog2e = 1.44269504088896340736f;
-// k of the row statistics
-__host__ __device__ inline float exp_scale(double temperature) { return (float)(1.44269504088896340736 / temperature); }
 #define NEG_INF (-__builtin_inff())
 
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// k = hi + lo of the row statistics.  One float for k is off by up to 2^-25,
+// always to the same side: lse would be off by that share of the mean |d|
+// (1e-7 for logits of a trained model, as much as float32's own rounding).
+// The other roundings are of either sign and average out over a row; so does
+// v_exp_f32's (mean -3e-9, at most 8e-8, measured over [-24, 0]).
+// hi is k rounded down and lo > 0, so that d = -inf gives -inf twice.
+struct ExpScale {
+    float hi, lo;
+};
+__host__ __device__ inline ExpScale exp_scale(double temperature) {
+    const double k = 1.44269504088896340736 / temperature;
+    float hi = (float)k;
+    if ((double)hi > k) hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, hi) - 1u);  // k > 0: one step down
+    const float lo = (float)(k - (double)hi);
+    return {hi, lo > 0.f ? lo : 1e-30f};
+}
+__device__ inline float exp2_scaled(float d, ExpScale k) { return exp2_hw(__builtin_fmaf(d, k.hi, d * k.lo)); }
 
 // 16 bytes of a row: N elements.
 template <typename T>
@@ -101,38 +116,69 @@ struct RowStat {
 
 // Joins b into a.  A side that is empty (m = -inf, s = 0) adds nothing; NaN
 // and +inf anywhere make s NaN.
-__device__ inline RowStat join(RowStat a, RowStat b, float k) {
+__device__ inline RowStat join(RowStat a, RowStat b, ExpScale k) {
     const float m = fmaxf(a.m, b.m);
     const float r = m == NEG_INF ? 0.f : m;
-    return {m, a.s * exp2_hw((a.m - r) * k) + b.s * exp2_hw((b.m - r) * k)};
+    return {m, a.s * exp2_scaled(a.m - r, k) + b.s * exp2_scaled(b.m - r, k)};
 }
 
-__device__ inline RowStat join_wave(RowStat a, float k) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        RowStat b{__shfl_xor(a.m, o), __shfl_xor(a.s, o)};
-        a = join(a, b, k);
-    }
-    return a;
-}
+// The block's maximum and sum, in every thread.  The maximum first: each
+// thread's sum is then scaled once, and the scaled sums are added in 64 bits.
+// Joining pairs level by level would round the last levels' few numbers again
+// and again: 1e-7 in lse, several times what the thread sums leave.
+struct BlockStat {
+    float m;
+    double s;
+};
 
-// The block's statistic, in every thread.
 template <int NT>
-__device__ inline RowStat join_block(RowStat a, float k, RowStat *lds) {
-    a = join_wave(a, k);
+struct BlockLds {
+    float m[NT / 64];
+    double s[NT / 64];
+};
+
+template <int NT>
+__device__ inline BlockStat join_block(RowStat a, ExpScale k, BlockLds<NT> &lds) {
     const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) lds[wave] = a;
-    __syncthreads();
-    RowStat r = lds[0];
+    float m = a.m;
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) r = join(r, lds[w], k);
-    return r;
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((threadIdx.x & 63) == 0) lds.m[wave] = m;
+    __syncthreads();
+    m = lds.m[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) m = fmaxf(m, lds.m[w]);
+    const float r = m == NEG_INF ? 0.f : m;
+    double s = (double)a.s * (double)exp2_scaled(a.m - r, k);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) lds.s[wave] = s;
+    __syncthreads();
+    s = lds.s[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) s += lds.s[w];
+    return {m, s};
+}
+
+// Terms are added to each other before they reach the running sum: one by
+// one, those below half its last bit would all be lost, and a vocabulary's
+// tail is many of them (3e-7 in lse at 131,072 classes).
+template <int N>
+__device__ inline float tree_sum(const float (&e)[N]) {
+    float t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = e[i];
+#pragma unroll
+    for (int w = N / 2; w; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) t[i] += t[i + w];
+    return t[0];
 }
 
 // One pass over a row: U packs a thread in flight, one rescaling of the
 // running sum per U packs.
 template <typename T, int NT, int U>
-__device__ inline RowStat row_stat(const T *row, int vocab, float k) {
+__device__ inline RowStat row_stat(const T *row, int vocab, ExpScale k) {
     using PK = Pack<T>;
     constexpr int N = PK::N;
     const int packs = vocab / N;
@@ -154,15 +200,19 @@ __device__ inline RowStat row_stat(const T *row, int vocab, float k) {
                 for (int i = 0; i < N; ++i) m = fmaxf(m, PK::get(v[u], i));
             }
         const float r = m == NEG_INF ? 0.f : m;
-        float s = a.s * exp2_hw((a.m - r) * k);
+        float s[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            s[u] = 0.f;
             if (have[u]) {
+                float e[N];
 #pragma unroll
-                for (int i = 0; i < N; ++i) s += exp2_hw((PK::get(v[u], i) - r) * k);
+                for (int i = 0; i < N; ++i) e[i] = exp2_scaled(PK::get(v[u], i) - r, k);
+                s[u] = tree_sum(e);
             }
+        }
+        a.s = a.s * exp2_scaled(a.m - r, k) + tree_sum(s);
         a.m = m;
-        a.s = s;
     }
     const int tail = packs * N + threadIdx.x;
     if (tail < vocab) {
@@ -182,8 +232,8 @@ __device__ inline double target_logprob(float zy, float m, double ln_s, double t
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t stride, int vocab, const void *target,
-                                                      int target_bits, float k, double tau, float *logprob, float *lse) {
-    __shared__ RowStat lds[NT / 64];
+                                                      int target_bits, ExpScale k, double tau, float *logprob, float *lse) {
+    __shared__ BlockLds<NT> lds;
     const int64_t t = blockIdx.x;
     const int64_t y = load_target(target, target_bits, t);
     if (y < 0) {  // ignored: the row is not read
@@ -195,9 +245,9 @@ __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t s
     }
     const T *row = logits + t * stride;
     const float zy = y < vocab ? (float)row[y] : __builtin_nanf("");
-    const RowStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
+    const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
     if (threadIdx.x == 0) {
-        const double ln = log((double)a.s);
+        const double ln = log(a.s);
         lse[t] = (float)(a.m / tau + ln);
         logprob[t] = (float)target_logprob(zy, a.m, ln, tau);
     }
@@ -269,17 +319,17 @@ __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int6
     const float c = y < vocab ? (float)(g / tau) : __builtin_nanf("");
     const float l = lse[t];
     if (fabsf(l) > kLseExact) {
-        __shared__ RowStat lds[NT / 64];
-        const float k = exp_scale(tau);
-        const RowStat a = join_block<NT>(row_stat<T, NT, 4>(logits + t * stride, vocab, k), k, lds);
-        const float neg = -c / a.s, m = a.m;
+        __shared__ BlockLds<NT> lds;
+        const ExpScale k = exp_scale(tau);
+        const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(logits + t * stride, vocab, k), k, lds);
+        const float neg = (float)(-c / a.s), m = a.m;
         residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
-                               [=](float z) { return neg * exp2_hw((z - m) * k); });
+                               [=](float z) { return neg * exp2_hw((z - m) * k.hi); });
         return;
     }
     const float it = (float)(1.0 / tau);
     residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
-                           [=](float z) { return -c * exp2_hw(__builtin_fmaf(z, it, -l) * kLog2e); });
+                           [=](float z) { return -c * exp2_hw(__builtin_fmaf(z, it, -l) * 1.44269504f); });
 }
 
 // ---------------------------------------------------------------- policy loss
@@ -320,9 +370,9 @@ __device__ inline double policy_token(double lp, const dlr_policy &p, int64_t t,
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t stride, int vocab, const void *target,
-                                                    int target_bits, float k, double tau, dlr_policy p, PolicyOut po,
+                                                    int target_bits, ExpScale k, double tau, dlr_policy p, PolicyOut po,
                                                     T *out, int64_t out_stride) {
-    __shared__ RowStat lds[NT / 64];
+    __shared__ BlockLds<NT> lds;
     __shared__ float coef;
     const int64_t t = blockIdx.x;
     const int64_t y = load_target(target, target_bits, t);
@@ -337,16 +387,16 @@ __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t str
     }
     const T *row = logits + t * stride;
     const float zy = y < vocab ? (float)row[y] : __builtin_nanf("");
-    const RowStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
+    const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
     if (threadIdx.x == 0) {
-        const double lp = target_logprob(zy, a.m, log((double)a.s), tau);
+        const double lp = target_logprob(zy, a.m, log(a.s), tau);
         coef = (float)(policy_token(lp, p, t, w, po) / tau);
     }
     if (!out) return;
     __syncthreads();
-    const float c = coef, neg = -c / a.s, m = a.m;
+    const float c = coef, neg = (float)(-c / a.s), m = a.m;
     residual_row<T, NT, 4>(row, out + t * out_stride, vocab, y, c,
-                           [=](float z) { return neg * exp2_hw((z - m) * k); });
+                           [=](float z) { return neg * exp2_hw((z - m) * k.hi); });
 }
 
 // ------------------------------------------------------------ preference loss
@@ -504,7 +554,7 @@ __global__ __launch_bounds__(256) void k_head_tile(dlr_head h, float2 *part, flo
                 for (int j = 0; j < 4; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
         }
     }
-    const float k = exp_scale(h.temperature);
+    const ExpScale k = exp_scale(h.temperature);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int64_t t = t0 + wt * 64 + j * 16 + (lane & 15);
@@ -539,19 +589,27 @@ __global__ __launch_bounds__(256) void k_head_join(dlr_head h, int64_t tiles, co
     if (t >= h.rows) return;
     const int lane = threadIdx.x & 63;
     const int64_t y = load_target(h.target, h.target_bits, t);
-    const float k = exp_scale(h.temperature);
-    RowStat a{NEG_INF, 0.f};
-    if (y >= 0)
+    const ExpScale k = exp_scale(h.temperature);
+    // the maximum first, then the scaled sums in 64 bits (as join_block)
+    float m = NEG_INF;
+    double sum = 0.0;
+    if (y >= 0) {
+        for (int64_t i = lane; i < tiles; i += 64) m = fmaxf(m, part[i * h.rows + t].x);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const float r = m == NEG_INF ? 0.f : m;
         for (int64_t i = lane; i < tiles; i += 64) {
             const float2 q = part[i * h.rows + t];
-            a = join(a, RowStat{q.x, q.y}, k);
+            sum += (double)q.y * (double)exp2_scaled(q.x - r, k);
         }
-    a = join_wave(a, k);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    }
     if (lane) return;
     const double tau = h.temperature;
-    const double ln = log((double)a.s);
-    lse[t] = y < 0 ? 0.f : (float)(a.m / tau + ln);
-    logprob[t] = y < 0 ? 0.f : y < h.vocab ? (float)target_logprob(zy[t], a.m, ln, tau) : __builtin_nanf("");
+    const double ln = log(sum);
+    lse[t] = y < 0 ? 0.f : (float)(m / tau + ln);
+    logprob[t] = y < 0 ? 0.f : y < h.vocab ? (float)target_logprob(zy[t], m, ln, tau) : __builtin_nanf("");
 }
 
 }  // namespace
