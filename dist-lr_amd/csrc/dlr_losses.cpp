@@ -60,6 +60,7 @@ bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
 constexpr int64_t kMaxRows = INT64_C(0x7fffffff);  // one workgroup per row
 constexpr int64_t kMaxVocab = INT64_C(1) << 30;
 constexpr int64_t kMaxDim = INT64_C(1) << 20;
+constexpr int64_t kMaxLogits = INT64_C(1) << 44;  // a head call's: its tiles are one launch
 
 const char *check_target(const void *target, int32_t bits, double temperature) {
     if (!target) return "target is NULL";
@@ -192,7 +193,8 @@ int dlr_preference_loss(int device, void *stream, const dlr_preference *p, float
 }
 
 int64_t dlr_head_logprob_workspace(int64_t rows, int64_t vocab, int64_t dim) {
-    if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || dim < 1 || dim > kMaxDim)
+    if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || dim < 1 || dim > kMaxDim ||
+        rows * vocab > kMaxLogits)
         return refuse(DLR_E_ARG, "dlr_head_logprob_workspace", "rows, vocab or dim is out of range");
     return dlr::head_workspace(rows, vocab);
 }
@@ -204,6 +206,7 @@ int dlr_head_logprob(int device, void *stream, const dlr_head *h, void *workspac
     if (h->rows < 0 || h->rows > kMaxRows) return refuse(DLR_E_ARG, call, "rows must be 0 .. 2^31 - 1");
     if (h->vocab < 1 || h->vocab > kMaxVocab) return refuse(DLR_E_ARG, call, "vocab must be 1 .. 2^30");
     if (h->dim < 1 || h->dim > kMaxDim) return refuse(DLR_E_ARG, call, "dim must be 1 .. 2^20");
+    if (h->rows * h->vocab > kMaxLogits) return refuse(DLR_E_ARG, call, "rows * vocab must be at most 2^44");
     if (h->dtype != DLR_DTYPE_BF16 && h->dtype != DLR_DTYPE_F16)
         return refuse(DLR_E_ARG, call, "dtype must be DLR_DTYPE_BF16 or DLR_DTYPE_F16");
     if (h->rows == 0) return DLR_OK;

@@ -526,7 +526,8 @@ __global__ __launch_bounds__(256) void k_head_tile(dlr_head h, float2 *part, flo
     __shared__ __attribute__((aligned(16))) uint16_t sx[kTileT * kLdsRow];
     __shared__ RowStat st[2][kTileT];
     const uint16_t *head = static_cast<const uint16_t *>(h.head), *hidden = static_cast<const uint16_t *>(h.hidden);
-    const int64_t v0 = (int64_t)blockIdx.x * kTileV, t0 = (int64_t)blockIdx.y * kTileT;
+    const int64_t vtiles = (h.vocab + kTileV - 1) / kTileV, vt = blockIdx.x % vtiles;
+    const int64_t v0 = vt * kTileV, t0 = blockIdx.x / vtiles * kTileT;
     const int dim = (int)h.dim;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wv = wave >> 1, wt = wave & 1;
     f32x4 acc[4][4] = {};
@@ -578,8 +579,141 @@ __global__ __launch_bounds__(256) void k_head_tile(dlr_head h, float2 *part, flo
     __syncthreads();
     if (tid < kTileT && t0 + tid < h.rows) {
         const RowStat a = join(st[0][tid], st[1][tid], k);
-        part[(int64_t)blockIdx.x * h.rows + t0 + tid] = make_float2(a.m, a.s);
+        part[vt * h.rows + t0 + tid] = make_float2(a.m, a.s);
     }
+}
+
+// ---- large tiles: both operands through LDS by DMA, double buffered
+//
+// A workgroup of 8 waves takes WV * 16 * MV classes x WT * 16 * MT tokens,
+// 64 of the dimension at a time.  Rows of a stage are 128 bytes; the 16-byte
+// chunk c of row r sits at slot c ^ swz(r), so that a wave's fragment reads
+// (16 rows, one chunk) spread over the banks although the DMA writes
+// linearly: the lane that fills slot s of row r fetches chunk s ^ swz(r).
+__device__ const u32x4 kZero16 = {0u, 0u, 0u, 0u};
+
+__device__ inline int swz(int r) { return r & 7; }
+
+// 64 lanes x 16 bytes, memory to LDS: lane i's at lds + 16 i.
+__device__ inline void lds_dma16(const void *src, void *lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                     (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+
+template <typename T, int WV, int WT, int MV, int MT>
+__global__ __launch_bounds__(512, 1) void k_head_big(dlr_head h, int vtiles, int ttiles, float2 *part, float *zy) {
+    constexpr int TV = WV * MV * 16, TT = WT * MT * 16, kRow = 128;
+    static_assert(WV * WT == 8 && TV % 64 == 0 && TT % 64 == 0, "8 waves, whole DMA loads");
+    constexpr int LV = TV / 64, LT = TT / 64;  // DMA loads a wave, 8 rows each
+    __shared__ __attribute__((aligned(256))) char sm[2][(TV + TT) * kRow];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wv = wave / WT, wt = wave % WT;
+    // XCD x takes a contiguous piece of the tile order, in which up to 8
+    // token tiles of one class tile follow each other: an XCD's 32 running
+    // workgroups share 8 token and 4 class tiles in its L2.
+    int64_t tile = blockIdx.x;
+    {
+        const int64_t n = (int64_t)vtiles * ttiles, q = n / 8, rem = n % 8, x = tile % 8;
+        tile = x * q + (x < rem ? x : rem) + tile / 8;
+    }
+    const int64_t group = (int64_t)vtiles * 8;  // tiles of 8 token tiles' group
+    const int64_t g = tile / group;
+    const int in_g = ttiles - g * 8 < 8 ? (int)(ttiles - g * 8) : 8;
+    const int64_t rest = tile - g * group;
+    const int64_t vt = rest / in_g, tt = g * 8 + rest % in_g;
+    const int64_t v0 = vt * TV, t0 = tt * TT;
+    const int dim = (int)h.dim, steps = (dim + 63) / 64;
+
+    // this lane's rows of the DMA loads; rows outside repeat the last one
+    const char *src[LV + LT];
+    const int chunk = (lane & 7) ^ swz(lane >> 3);
+#pragma unroll
+    for (int q = 0; q < LV + LT; ++q) {
+        const bool x = q >= LV;
+        const int r = x ? (wave * LT + q - LV) * 8 + (lane >> 3) : (wave * LV + q) * 8 + (lane >> 3);
+        int64_t row = (x ? t0 : v0) + r;
+        const int64_t last = (x ? h.rows : h.vocab) - 1;
+        row = row < last ? row : last;
+        src[q] = static_cast<const char *>(x ? h.hidden : h.head) + row * (x ? h.hidden_stride : h.head_stride) * 2 +
+                 chunk * 16;
+    }
+    auto fill = [&](int step, int buf) {
+        char *dst = sm[buf];
+        const bool in = step * 64 + chunk * 8 < dim;  // dim is a multiple of 8
+#pragma unroll
+        for (int q = 0; q < LV + LT; ++q) {
+            const int at = q >= LV ? TV * kRow + (wave * LT + q - LV) * 1024 : (wave * LV + q) * 1024;
+            const void *s = src[q] + (int64_t)step * 128;
+            lds_dma16(in ? s : (const void *)&kZero16, dst + at);
+        }
+    };
+    f32x4 acc[MV][MT] = {};
+    fill(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    for (int step = 0; step < steps; ++step) {
+        const int buf = step & 1;
+        if (step + 1 < steps) fill(step + 1, buf ^ 1);
+        const char *sv = sm[buf] + (wv * MV * 16 + (lane & 15)) * kRow;
+        const char *st = sm[buf] + TV * kRow + (wt * MT * 16 + (lane & 15)) * kRow;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const int slot = ((ks * 4 + (lane >> 4)) ^ swz(lane & 15)) * 16;  // rows 16 apart have the same swz
+            u32x4 a[MV], b[MT];
+#pragma unroll
+            for (int j = 0; j < MT; ++j) b[j] = *reinterpret_cast<const u32x4 *>(st + j * 16 * kRow + slot);
+#pragma unroll
+            for (int i = 0; i < MV; ++i) a[i] = *reinterpret_cast<const u32x4 *>(sv + i * 16 * kRow + slot);
+#pragma unroll
+            for (int i = 0; i < MV; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the next stage has landed
+        __syncthreads();
+    }
+    // per token (a lane column) over this wave's classes, then over the waves
+    const ExpScale k = exp_scale(h.temperature);
+    RowStat *stat = reinterpret_cast<RowStat *>(sm[0]);  // [WV][TT]
+    const bool ragged = v0 + TV > h.vocab;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int64_t t = t0 + wt * MT * 16 + j * 16 + (lane & 15);
+        const int64_t y = t < h.rows ? load_target(h.target, h.target_bits, t) : -1;
+        const int64_t base = v0 + wv * MV * 16 + (lane >> 4) * 4;
+        float m = NEG_INF;
+#pragma unroll
+        for (int i = 0; i < MV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (ragged && base + i * 16 + e >= h.vocab) acc[i][j][e] = NEG_INF;
+                if (base + i * 16 + e == y) zy[t] = acc[i][j][e];
+                m = fmaxf(m, acc[i][j][e]);
+            }
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const float r = m == NEG_INF ? 0.f : m;
+        float s[MV];
+#pragma unroll
+        for (int i = 0; i < MV; ++i) {
+            float e4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) e4[e] = exp2_scaled(acc[i][j][e] - r, k);
+            s[i] = tree_sum(e4);
+        }
+        float sum = tree_sum(s);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (lane < 16) stat[wv * TT + wt * MT * 16 + j * 16 + lane] = {m, sum};
+    }
+    __syncthreads();
+    for (int i = tid; i < TT; i += 512)
+        if (t0 + i < h.rows) {
+            RowStat a = stat[i];
+#pragma unroll
+            for (int w = 1; w < WV; ++w) a = join(a, stat[w * TT + i], k);
+            part[vt * h.rows + t0 + i] = make_float2(a.m, a.s);
+        }
 }
 
 // The tiles' statistics of one token, joined by one wave.
@@ -660,20 +794,37 @@ hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float
     return hipGetLastError();
 }
 
+// The classes of a tile of the kernel that launch_head_logprob takes.
+static int head_tile(const dlr_head &h) {
+    const bool even = (reinterpret_cast<uintptr_t>(h.head) | reinterpret_cast<uintptr_t>(h.hidden)) % 16 == 0 &&
+                      h.head_stride % 8 == 0 && h.hidden_stride % 8 == 0 && h.dim % 8 == 0;
+    return even ? 256 : kTileV;
+}
+
 int64_t head_workspace(int64_t rows, int64_t vocab) {
     const int64_t tiles = (vocab + kTileV - 1) / kTileV;
-    return rows * tiles * (int64_t)sizeof(float2) + rows * (int64_t)sizeof(float);
+    return rows * tiles * (int64_t)sizeof(float2) + (rows + 1) / 2 * 2 * (int64_t)sizeof(float);
+}
+
+template <typename T>
+static int64_t launch_head_tiles(hipStream_t st, const dlr_head &h, float2 *part, float *zy) {
+    const int tv = head_tile(h);
+    const int64_t vtiles = (h.vocab + tv - 1) / tv;
+    if (tv == 256) {
+        const int64_t ttiles = (h.rows + 255) / 256;
+        k_head_big<T, 2, 4, 8, 4><<<dim3((unsigned)(vtiles * ttiles)), 512, 0, st>>>(h, (int)vtiles, (int)ttiles, part, zy);
+    } else {
+        k_head_tile<T><<<dim3((unsigned)(vtiles * ((h.rows + kTileT - 1) / kTileT))), 256, 0, st>>>(h, part, zy);
+    }
+    return vtiles;
 }
 
 hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
-    const int64_t tiles = (h.vocab + kTileV - 1) / kTileV;
-    float2 *part = static_cast<float2 *>(workspace);
-    float *zy = reinterpret_cast<float *>(part + tiles * h.rows);
-    const dim3 grid((unsigned)tiles, (unsigned)((h.rows + kTileT - 1) / kTileT));
-    if (h.dtype == DLR_DTYPE_BF16)
-        k_head_tile<__bf16><<<grid, 256, 0, st>>>(h, part, zy);
-    else
-        k_head_tile<_Float16><<<grid, 256, 0, st>>>(h, part, zy);
+    // zy first: its place does not depend on the kernel's tiles
+    float *zy = static_cast<float *>(workspace);
+    float2 *part = reinterpret_cast<float2 *>(zy + (h.rows + 1) / 2 * 2);
+    const int64_t tiles = h.dtype == DLR_DTYPE_BF16 ? launch_head_tiles<__bf16>(st, h, part, zy)
+                                                    : launch_head_tiles<_Float16>(st, h, part, zy);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     k_head_join<<<dim3((unsigned)((h.rows + 3) / 4)), 256, 0, st>>>(h, tiles, part, zy, logprob, lse);

@@ -743,7 +743,7 @@ typedef struct dlr_head {
     const void *hidden;         /* rows x dim                                 */
     const void *head;           /* vocab x dim: one row of weights per class  */
     const void *target;
-    int64_t rows, vocab, dim;   /* dim 1 .. 2^20                              */
+    int64_t rows, vocab, dim;   /* dim 1 .. 2^20, rows * vocab <= 2^44        */
     int64_t hidden_stride;      /* elements between rows                      */
     int64_t head_stride;
     int32_t dtype;

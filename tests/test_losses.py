@@ -125,6 +125,7 @@ def test_preference_gradient_over_an_input():
 
 @pytest.mark.parametrize("kw,word", [
     (dict(rows=-1), "rows"), (dict(vocab=0), "vocab"), (dict(dim=0), "dim"), (dict(dim=(1 << 20) + 1), "dim"),
+    (dict(rows=1 << 30, vocab=1 << 20), "rows"),
     (dict(dtype=L.DTYPE_F32), "dtype"), (dict(hidden=None), "NULL"), (dict(head=A + 1), "aligned"),
     (dict(hidden_stride=63), "hidden_stride"), (dict(head_stride=63), "head_stride"), (dict(head_stride=0), "head_stride"),
     (dict(target=None), "target"), (dict(temperature=0.0), "temperature")])
