@@ -583,16 +583,15 @@ __global__ __launch_bounds__(256) void k_head_tile(dlr_head h, float2 *part, flo
     }
 }
 
-// ---- large tiles: both operands through LDS by DMA, double buffered
+// ---- aligned rows: both operands through LDS by DMA
 //
-// A workgroup of 8 waves takes WV * 16 * MV classes x WT * 16 * MT tokens,
-// 64 of the dimension at a time.  Rows of a stage are 128 bytes; the 16-byte
-// chunk c of row r sits at slot c ^ swz(r), so that a wave's fragment reads
-// (16 rows, one chunk) spread over the banks although the DMA writes
-// linearly: the lane that fills slot s of row r fetches chunk s ^ swz(r).
+// A workgroup of WV x WT waves takes TV = WV * 16 * MV classes x TT = WT * 16
+// * MT tokens, 64 of the dimension (a stage) at a time, S stages in LDS.
+// Rows of a stage are 128 bytes, classes first; the 16-byte chunk c of row r
+// sits at slot c ^ (r & 7), so that a wave's fragment reads (16 rows, one
+// chunk) meet no bank twice although the DMA writes linearly: the lane that
+// fills slot s of row r fetches chunk s ^ (r & 7).
 __device__ const u32x4 kZero16 = {0u, 0u, 0u, 0u};
-
-__device__ inline int swz(int r) { return r & 7; }
 
 // 64 lanes x 16 bytes, memory to LDS: lane i's at lds + 16 i.
 __device__ inline void lds_dma16(const void *src, void *lds) {
@@ -600,12 +599,19 @@ __device__ inline void lds_dma16(const void *src, void *lds) {
                                      (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
 }
 
-template <typename T, int WV, int WT, int MV, int MT>
-__global__ __launch_bounds__(512, 1) void k_head_big(dlr_head h, int vtiles, int ttiles, float2 *part, float *zy) {
-    constexpr int TV = WV * MV * 16, TT = WT * MT * 16, kRow = 128;
-    static_assert(WV * WT == 8 && TV % 64 == 0 && TT % 64 == 0, "8 waves, whole DMA loads");
-    constexpr int LV = TV / 64, LT = TT / 64;  // DMA loads a wave, 8 rows each
-    __shared__ __attribute__((aligned(256))) char sm[2][(TV + TT) * kRow];
+// One scheduling group: N instructions of a kind (8: MFMA, 32: memory reads,
+// 256: LDS reads), in program order with the groups around it.
+#define SCHED_MFMA(n) __builtin_amdgcn_sched_group_barrier(8, n, 0)
+#define SCHED_DMA(n) __builtin_amdgcn_sched_group_barrier(32, n, 0)
+#define SCHED_LDS(n) __builtin_amdgcn_sched_group_barrier(256, n, 0)
+
+template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
+__global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int vtiles, int ttiles, float2 *part,
+                                                               float *zy) {
+    constexpr int NW = WV * WT, TV = WV * MV * 16, TT = WT * MT * 16, kRow = 128;
+    constexpr int kLoads = (TV + TT) / 8, L = (kLoads + NW - 1) / NW;  // DMA loads of 8 rows: all, a wave's
+    static_assert(TV % 8 == 0 && TT % 8 == 0 && S >= 2 && L * (S - 2) < 64, "whole loads, a wait that can be written");
+    __shared__ __attribute__((aligned(256))) char sm[S][(TV + TT) * kRow];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wv = wave / WT, wt = wave % WT;
     // XCD x takes a contiguous piece of the tile order, in which up to 8
@@ -622,56 +628,115 @@ __global__ __launch_bounds__(512, 1) void k_head_big(dlr_head h, int vtiles, int
     const int64_t rest = tile - g * group;
     const int64_t vt = rest / in_g, tt = g * 8 + rest % in_g;
     const int64_t v0 = vt * TV, t0 = tt * TT;
-    const int dim = (int)h.dim, steps = (dim + 63) / 64;
+    const int dim = (int)h.dim, full = dim / 64, steps = (dim + 63) / 64;
 
-    // this lane's rows of the DMA loads; rows outside repeat the last one
-    const char *src[LV + LT];
-    const int chunk = (lane & 7) ^ swz(lane >> 3);
+    // This lane's places in the wave's DMA loads, from the tile's first row.
+    // Rows outside repeat the last one; a wave without an L-th load repeats
+    // the last load (every wave then has L of them in flight per stage).
+    const char *base_v = static_cast<const char *>(h.head) + v0 * h.head_stride * 2;
+    const char *base_t = static_cast<const char *>(h.hidden) + t0 * h.hidden_stride * 2;
+    uint32_t off[L];
+    const int chunk = (lane & 7) ^ (lane >> 3);
+    auto load_no = [&](int q) {
+        const int n = wave * L + q;
+        return n < kLoads ? n : kLoads - 1;
+    };
 #pragma unroll
-    for (int q = 0; q < LV + LT; ++q) {
-        const bool x = q >= LV;
-        const int r = x ? (wave * LT + q - LV) * 8 + (lane >> 3) : (wave * LV + q) * 8 + (lane >> 3);
-        int64_t row = (x ? t0 : v0) + r;
-        const int64_t last = (x ? h.rows : h.vocab) - 1;
-        row = row < last ? row : last;
-        src[q] = static_cast<const char *>(x ? h.hidden : h.head) + row * (x ? h.hidden_stride : h.head_stride) * 2 +
-                 chunk * 16;
+    for (int q = 0; q < L; ++q) {
+        const int n = load_no(q);
+        const bool x = n >= TV / 8;
+        const int r = (x ? n - TV / 8 : n) * 8 + (lane >> 3);
+        const int64_t last = x ? h.rows - 1 - t0 : h.vocab - 1 - v0;
+        off[q] = (uint32_t)((r < last ? r : last) * (x ? h.hidden_stride : h.head_stride) * 2 + chunk * 16);
     }
     auto fill = [&](int step, int buf) {
-        char *dst = sm[buf];
-        const bool in = step * 64 + chunk * 8 < dim;  // dim is a multiple of 8
+        const char *sv = base_v + (int64_t)step * 128, *st = base_t + (int64_t)step * 128;
 #pragma unroll
-        for (int q = 0; q < LV + LT; ++q) {
-            const int at = q >= LV ? TV * kRow + (wave * LT + q - LV) * 1024 : (wave * LV + q) * 1024;
-            const void *s = src[q] + (int64_t)step * 128;
-            lds_dma16(in ? s : (const void *)&kZero16, dst + at);
-        }
+        for (int q = 0; q < L; ++q) lds_dma16((load_no(q) >= TV / 8 ? st : sv) + off[q], sm[buf] + load_no(q) * 1024);
+    };
+    auto fill_last = [&](int step, int buf) {  // a stage that may be short (dim is a multiple of 8): zeros behind it
+        const bool in = step * 64 + chunk * 8 < dim;
+        const char *sv = base_v + (int64_t)step * 128, *st = base_t + (int64_t)step * 128;
+#pragma unroll
+        for (int q = 0; q < L; ++q)
+            lds_dma16(in ? (load_no(q) >= TV / 8 ? st : sv) + off[q] : (const char *)&kZero16,
+                      sm[buf] + load_no(q) * 1024);
+    };
+    struct Frag {
+        u32x4 a[MV], b[MT];
+    };
+    const int at_v = (wv * MV * 16 + (lane & 15)) * kRow, at_t = TV * kRow + (wt * MT * 16 + (lane & 15)) * kRow;
+    auto read = [&](Frag &f, int buf, int half) {
+        const int slot = ((half * 4 + (lane >> 4)) ^ (lane & 7)) * 16;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) f.b[j] = *reinterpret_cast<const u32x4 *>(sm[buf] + at_t + j * 16 * kRow + slot);
+#pragma unroll
+        for (int i = 0; i < MV; ++i) f.a[i] = *reinterpret_cast<const u32x4 *>(sm[buf] + at_v + i * 16 * kRow + slot);
     };
     f32x4 acc[MV][MT] = {};
-    fill(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    for (int step = 0; step < steps; ++step) {
-        const int buf = step & 1;
-        if (step + 1 < steps) fill(step + 1, buf ^ 1);
-        const char *sv = sm[buf] + (wv * MV * 16 + (lane & 15)) * kRow;
-        const char *st = sm[buf] + TV * kRow + (wt * MT * 16 + (lane & 15)) * kRow;
+    auto multiply = [&](const Frag &f) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const int slot = ((ks * 4 + (lane >> 4)) ^ swz(lane & 15)) * 16;  // rows 16 apart have the same swz
-            u32x4 a[MV], b[MT];
+        for (int i = 0; i < MV; ++i)
 #pragma unroll
-            for (int j = 0; j < MT; ++j) b[j] = *reinterpret_cast<const u32x4 *>(st + j * 16 * kRow + slot);
+            for (int j = 0; j < MT; ++j) acc[i][j] = mfma(f.a[i], f.b[j], acc[i][j], T());
+    };
+    // The first half's fragments of a stage are read while the second half
+    // of the stage before is multiplied, the second half's while the first
+    // is: the matrix cores wait for LDS nowhere.  One barrier a stage, in its
+    // middle: then the next stage has landed (each wave waits for its own
+    // part first; `later` loads of the stages behind it stay in flight) and
+    // nobody reads this one any more.
+#define MEET(later)                                                                                \
+    do {                                                                                           \
+        __builtin_amdgcn_sched_barrier(0);                                                         \
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(later) : "memory");                    \
+        __builtin_amdgcn_s_barrier();                                                              \
+        asm volatile("" ::: "memory");                                                             \
+    } while (0)
+    Frag f0, f1;
 #pragma unroll
-            for (int i = 0; i < MV; ++i) a[i] = *reinterpret_cast<const u32x4 *>(sv + i * 16 * kRow + slot);
+    for (int p = 0; p < S; ++p)
+        if (p < steps) fill_last(p, p);
+    MEET(0);
+    read(f0, 0, 0);
+    int step = 0, buf = 0;
+    for (; step + S < full; ++step) {
+        const int next = buf + 1 < S ? buf + 1 : 0;
+        read(f1, buf, 1);
+        multiply(f0);
 #pragma unroll
-            for (int i = 0; i < MV; ++i)
-#pragma unroll
-                for (int j = 0; j < MT; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j], T());
+        for (int i = 0; i < MV + MT; ++i) {
+            SCHED_LDS(1);
+            SCHED_MFMA(2);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the next stage has landed
-        __syncthreads();
+        MEET(L *(S - 2));
+        fill(step + S, buf);
+        read(f0, next, 0);
+        multiply(f1);
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            SCHED_DMA(1);
+            SCHED_MFMA(2);
+        }
+#pragma unroll
+        for (int i = 0; i < MV + MT; ++i) {
+            SCHED_LDS(1);
+            SCHED_MFMA(1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        buf = next;
     }
+    for (; step < steps; ++step) {
+        const int next = buf + 1 < S ? buf + 1 : 0;
+        read(f1, buf, 1);
+        multiply(f0);
+        MEET(0);
+        if (step + S < steps) fill_last(step + S, buf);
+        if (step + 1 < steps) read(f0, next, 0);
+        multiply(f1);
+        buf = next;
+    }
+    __syncthreads();  // sm is free
     // per token (a lane column) over this wave's classes, then over the waves
     const ExpScale k = exp_scale(h.temperature);
     RowStat *stat = reinterpret_cast<RowStat *>(sm[0]);  // [WV][TT]
@@ -707,7 +772,7 @@ __global__ __launch_bounds__(512, 1) void k_head_big(dlr_head h, int vtiles, int
         if (lane < 16) stat[wv * TT + wt * MT * 16 + j * 16 + lane] = {m, sum};
     }
     __syncthreads();
-    for (int i = tid; i < TT; i += 512)
+    for (int i = tid; i < TT; i += NW * 64)
         if (t0 + i < h.rows) {
             RowStat a = stat[i];
 #pragma unroll
@@ -716,34 +781,53 @@ __global__ __launch_bounds__(512, 1) void k_head_big(dlr_head h, int vtiles, int
         }
 }
 
-// The tiles' statistics of one token, joined by one wave.
+// The tiles' statistics, joined: RT tokens a workgroup (their statistics lie
+// side by side), 256 / RT threads each.  The maximum first, then the scaled
+// sums in 64 bits (as join_block); a thread keeps its first 16 tiles.
+template <int RT>
 __global__ __launch_bounds__(256) void k_head_join(dlr_head h, int64_t tiles, const float2 *part, const float *zy,
                                                    float *logprob, float *lse) {
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= h.rows) return;
-    const int lane = threadIdx.x & 63;
-    const int64_t y = load_target(h.target, h.target_bits, t);
+    constexpr int G = 256 / RT, K = 16;
+    __shared__ float lm[4][RT];
+    __shared__ double ls[4][RT];
+    const int tok = threadIdx.x % RT, first = threadIdx.x / RT, wave = threadIdx.x >> 6;
+    const int64_t t = (int64_t)blockIdx.x * RT + tok;
+    const int64_t y = t < h.rows ? load_target(h.target, h.target_bits, t) : -1;
     const ExpScale k = exp_scale(h.temperature);
-    // the maximum first, then the scaled sums in 64 bits (as join_block)
-    float m = NEG_INF;
-    double sum = 0.0;
-    if (y >= 0) {
-        for (int64_t i = lane; i < tiles; i += 64) m = fmaxf(m, part[i * h.rows + t].x);
+    const float2 *p = part + (t < h.rows ? t : 0);
+    float2 q[K];
 #pragma unroll
-        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const float r = m == NEG_INF ? 0.f : m;
-        for (int64_t i = lane; i < tiles; i += 64) {
-            const float2 q = part[i * h.rows + t];
-            sum += (double)q.y * (double)exp2_scaled(q.x - r, k);
-        }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    for (int i = 0; i < K; ++i) {
+        const int64_t n = first + i * G;
+        q[i] = n < tiles ? p[n * h.rows] : make_float2(NEG_INF, 0.f);
     }
-    if (lane) return;
-    const double tau = h.temperature;
-    const double ln = log(sum);
+    const float z = y >= 0 && y < h.vocab ? zy[t] : __builtin_nanf("");
+    float m = NEG_INF;
+#pragma unroll
+    for (int i = 0; i < K; ++i) m = fmaxf(m, q[i].x);
+    for (int64_t n = first + K * G; n < tiles; n += G) m = fmaxf(m, p[n * h.rows].x);
+#pragma unroll
+    for (int o = RT; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((threadIdx.x & 63) < RT) lm[wave][tok] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(lm[0][tok], lm[1][tok]), fmaxf(lm[2][tok], lm[3][tok]));
+    const float r = m == NEG_INF ? 0.f : m;
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) s += (double)q[i].y * (double)exp2_scaled(q[i].x - r, k);
+    for (int64_t n = first + K * G; n < tiles; n += G) {
+        const float2 v = p[n * h.rows];
+        s += (double)v.y * (double)exp2_scaled(v.x - r, k);
+    }
+#pragma unroll
+    for (int o = RT; o < 64; o <<= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) < RT) ls[wave][tok] = s;
+    __syncthreads();
+    if (first || t >= h.rows) return;
+    s = (ls[0][tok] + ls[1][tok]) + (ls[2][tok] + ls[3][tok]);
+    const double tau = h.temperature, ln = log(s);
     lse[t] = y < 0 ? 0.f : (float)(m / tau + ln);
-    logprob[t] = y < 0 ? 0.f : y < h.vocab ? (float)target_logprob(zy[t], m, ln, tau) : __builtin_nanf("");
+    logprob[t] = y < 0 ? 0.f : (float)target_logprob(z, m, ln, tau);
 }
 
 }  // namespace
@@ -794,29 +878,60 @@ hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float
     return hipGetLastError();
 }
 
-// The classes of a tile of the kernel that launch_head_logprob takes.
-static int head_tile(const dlr_head &h) {
-    const bool even = (reinterpret_cast<uintptr_t>(h.head) | reinterpret_cast<uintptr_t>(h.hidden)) % 16 == 0 &&
-                      h.head_stride % 8 == 0 && h.hidden_stride % 8 == 0 && h.dim % 8 == 0;
-    return even ? 256 : kTileV;
+// Whether the rows can go through the DMA kernels: 16-byte chunks of rows
+// that start at 16 bytes, 32-bit places within a tile.
+static bool head_by_dma(const dlr_head &h) {
+    return (reinterpret_cast<uintptr_t>(h.head) | reinterpret_cast<uintptr_t>(h.hidden)) % 16 == 0 &&
+           h.head_stride % 8 == 0 && h.hidden_stride % 8 == 0 && h.dim % 8 == 0 && h.head_stride <= (1 << 21) &&
+           h.hidden_stride <= (1 << 21);
 }
 
+constexpr int kSmallestTile = 64;  // classes: the most tiles, for the workspace
+
 int64_t head_workspace(int64_t rows, int64_t vocab) {
-    const int64_t tiles = (vocab + kTileV - 1) / kTileV;
+    const int64_t tiles = (vocab + kSmallestTile - 1) / kSmallestTile;
     return rows * tiles * (int64_t)sizeof(float2) + (rows + 1) / 2 * 2 * (int64_t)sizeof(float);
 }
 
+template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
+static int64_t launch_head_dma(hipStream_t st, const dlr_head &h, float2 *part, float *zy) {
+    constexpr int TV = WV * MV * 16, TT = WT * MT * 16;
+    static_assert(TV >= kSmallestTile, "the workspace counts on it");
+    const int64_t vtiles = (h.vocab + TV - 1) / TV, ttiles = (h.rows + TT - 1) / TT;
+    k_head_dma<T, WV, WT, MV, MT, S, OCC><<<dim3((unsigned)(vtiles * ttiles)), WV * WT * 64, 0, st>>>(
+        h, (int)vtiles, (int)ttiles, part, zy);
+    return vtiles;
+}
+
+// The tile.  Up to 16 rows the head's bytes are all there is: 256 classes a
+// workgroup once that is two workgroups a CU, else 64 with a deeper queue
+// (1 row x 4096: 131,072 classes 180 us against 190, 65,536 classes 105
+// against 118).  Beyond, the cheapest by rounds of the 256 CUs, in units of a
+// 256 x 256 tile's time (80 us at dim 4096; the others' as measured there
+// alone on a CU and two on one): 256 x 256 runs at 1,360 TFLOP/s full, 256 x
+// 128 at 1,195, and the small ones fill the CUs where those cannot (200 x
+// 4096 x 32000: 63 us by 256 x 128, 95 by 256 x 256; 2048 x 4096 x 1000: 30
+// us by 128 x 64, 81).
 template <typename T>
 static int64_t launch_head_tiles(hipStream_t st, const dlr_head &h, float2 *part, float *zy) {
-    const int tv = head_tile(h);
-    const int64_t vtiles = (h.vocab + tv - 1) / tv;
-    if (tv == 256) {
-        const int64_t ttiles = (h.rows + 255) / 256;
-        k_head_big<T, 2, 4, 8, 4><<<dim3((unsigned)(vtiles * ttiles)), 512, 0, st>>>(h, (int)vtiles, (int)ttiles, part, zy);
-    } else {
+    if (!head_by_dma(h)) {
+        const int64_t vtiles = (h.vocab + kTileV - 1) / kTileV;
         k_head_tile<T><<<dim3((unsigned)(vtiles * ((h.rows + kTileT - 1) / kTileT))), 256, 0, st>>>(h, part, zy);
+        return vtiles;
     }
-    return vtiles;
+    constexpr int64_t kCus = 256;
+    if (h.rows <= 16)
+        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, part, zy)
+                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, part, zy);
+    auto tiles = [&](int64_t tv, int64_t tt) { return ((h.vocab + tv - 1) / tv) * ((h.rows + tt - 1) / tt); };
+    auto rounds = [&](int64_t n, int64_t slots) { return (double)((n + slots - 1) / slots); };
+    auto pair = [&](int64_t n, double alone, double two) { return n <= kCus ? alone : two * rounds(n, 2 * kCus); };
+    const double a = rounds(tiles(256, 256), kCus), b = 0.6 * rounds(tiles(256, 128), kCus),
+                 c = pair(tiles(128, 64), 0.35, 0.41), d = pair(tiles(64, 64), 0.27, 0.4);
+    if (a <= b && a <= c && a <= d) return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, part, zy);
+    if (b <= c && b <= d) return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, part, zy);
+    if (c <= d) return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, part, zy);
+    return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, part, zy);
 }
 
 hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
@@ -827,7 +942,10 @@ hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspac
                                                     : launch_head_tiles<_Float16>(st, h, part, zy);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_head_join<<<dim3((unsigned)((h.rows + 3) / 4)), 256, 0, st>>>(h, tiles, part, zy, logprob, lse);
+    if (h.rows < 16)
+        k_head_join<1><<<dim3((unsigned)h.rows), 256, 0, st>>>(h, tiles, part, zy, logprob, lse);
+    else
+        k_head_join<16><<<dim3((unsigned)((h.rows + 15) / 16)), 256, 0, st>>>(h, tiles, part, zy, logprob, lse);
     return hipGetLastError();
 }
 

@@ -88,30 +88,33 @@ def _refuse(why: str):
     raise DLRError(E_ARG, why)
 
 
-def _gpu(name: str, t) -> torch.device:
+def _gpu(name: str, t) -> int:
+    """The index of the tensor's GPU."""
     if not isinstance(t, torch.Tensor):
         _refuse(f"{name} must be a torch tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         _refuse(f"{name} must be on a GPU (it is on {t.device})")
-    return t.device
+    return t.get_device()
 
 
-def _matrix(name: str, t: torch.Tensor) -> None:
+def _matrix(name: str, t: torch.Tensor, gpu: int) -> None:
+    if _gpu(name, t) != gpu:
+        _refuse(f"{name} is on GPU {t.get_device()}, not on GPU {gpu}")
     if t.dim() != 2:
         _refuse(f"{name} must have 2 dimensions (it has {t.dim()})")
     if t.stride(1) != 1 and t.shape[1] > 1:
         _refuse(f"{name} must be contiguous within a row")
 
 
-def _vector(name: str, t, device: torch.device, dtypes, length: int) -> torch.Tensor:
+def _vector(name: str, t, gpu: int, dtypes, length: int) -> torch.Tensor:
     """A 1-D tensor of one of `dtypes`; a strided one is copied."""
-    if _gpu(name, t) != device:
-        _refuse(f"{name} is on {t.device}, not on {device}")
+    if _gpu(name, t) != gpu:
+        _refuse(f"{name} is on GPU {t.get_device()}, not on GPU {gpu}")
     if t.dtype not in dtypes:
         _refuse(f"{name} must be {' or '.join(str(d) for d in dtypes)} (it is {t.dtype})")
     if t.dim() != 1 or t.shape[0] != length:
         _refuse(f"{name} must have shape ({length},) (it has {tuple(t.shape)})")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 _F32 = (torch.float32,)
@@ -124,27 +127,34 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _logits(logits: torch.Tensor, target: torch.Tensor, temperature: float):
-    device = _gpu("logits", logits)
-    _matrix("logits", logits)
+    gpu = _gpu("logits", logits)
+    _matrix("logits", logits, gpu)
     if logits.dtype not in _DTYPES:
         _refuse(f"logits must be float32, bfloat16 or float16 (they are {logits.dtype})")
     rows, vocab = logits.shape
-    target = _vector("target", target, device, _INTS, rows)
-    return device, target, _Logits(logits.data_ptr(), target.data_ptr(), rows, vocab, logits.stride(0),
-                                   _DTYPES[logits.dtype], _TARGET_BITS[target.dtype], temperature)
+    target = _vector("target", target, gpu, _INTS, rows)
+    return gpu, target, _Logits(logits.data_ptr(), target.data_ptr(), rows, vocab, logits.stride(0),
+                                _DTYPES[logits.dtype], _TARGET_BITS[target.dtype], temperature)
 
 
-def _grad_like(logits: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+def _grad_like(logits: torch.Tensor, out: Optional[torch.Tensor], gpu: int) -> torch.Tensor:
     if out is None:
         return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    if _gpu("out", out) != logits.device or out.dtype != logits.dtype or out.shape != logits.shape:
-        _refuse("out must have the logits' device, type and shape")
-    _matrix("out", out)
+    _matrix("out", out, gpu)
+    if out.dtype != logits.dtype or out.shape != logits.shape:
+        _refuse("out must have the logits' type and shape")
     return out
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _rows(count: int, length: int, like: torch.Tensor):
+    """`count` float32 vectors side by side in one allocation, and its address."""
+    out = torch.empty((count, length), dtype=torch.float32, device=like.device)
+    return out.unbind(0), out.data_ptr()
+
+
+# The current stream of a GPU as an address: torch.cuda.current_stream(gpu).
+# cuda_stream without the Stream object, 2 us of a 10 us call.
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def token_logprob(logits: torch.Tensor, target: torch.Tensor, *,
@@ -153,11 +163,10 @@ def token_logprob(logits: torch.Tensor, target: torch.Tensor, *,
     temperature - lse, lse = log sum exp(logits[t] / temperature).  A
     negative target marks a row that takes no part: 0, not read
     (dlr_token_logprob)."""
-    device, target, x = _logits(logits, target, temperature)
-    out = torch.empty((2, x.rows), dtype=torch.float32, device=device)
-    logprob, lse = out[0], out[1]
-    _check(lib.dlr_token_logprob(device.index, _stream(device), C.byref(x), logprob.data_ptr(), lse.data_ptr()))
-    return logprob, lse
+    gpu, target, x = _logits(logits, target, temperature)
+    out, at = _rows(2, x.rows, logits)
+    _check(lib.dlr_token_logprob(gpu, _stream(gpu), C.byref(x), at, at + 4 * x.rows))
+    return out
 
 
 def token_logprob_grad(logits: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor, *,
@@ -166,11 +175,11 @@ def token_logprob_grad(logits: torch.Tensor, target: torch.Tensor, lse: torch.Te
     logits' type; lse is token_logprob's.  Rows with a negative target or
     grad 0 are 0.  out may be the logits themselves
     (dlr_token_logprob_grad)."""
-    device, target, x = _logits(logits, target, temperature)
-    lse = _vector("lse", lse, device, _F32, x.rows)
-    grad = _vector("grad", grad, device, _F32, x.rows)
-    out = _grad_like(logits, out)
-    _check(lib.dlr_token_logprob_grad(device.index, _stream(device), C.byref(x), lse.data_ptr(), grad.data_ptr(),
+    gpu, target, x = _logits(logits, target, temperature)
+    lse = _vector("lse", lse, gpu, _F32, x.rows)
+    grad = _vector("grad", grad, gpu, _F32, x.rows)
+    out = _grad_like(logits, out, gpu)
+    _check(lib.dlr_token_logprob_grad(gpu, _stream(gpu), C.byref(x), lse.data_ptr(), grad.data_ptr(),
                                       out.data_ptr(), out.stride(0)))
     return out
 
@@ -189,23 +198,23 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logprob: torch.T
     each row its share of a mean.  Rows with a negative target or weight 0
     take no part.  clipped: where the clip holds the surrogate.  out: the
     gradient's tensor, which may be the logits themselves."""
-    device, target, x = _logits(logits, target, temperature)
-    old_logprob = _vector("old_logprob", old_logprob, device, _F32, x.rows)
-    advantage = _vector("advantage", advantage, device, _F32, x.rows)
+    gpu, target, x = _logits(logits, target, temperature)
+    rows = x.rows
+    old_logprob = _vector("old_logprob", old_logprob, gpu, _F32, rows)
+    advantage = _vector("advantage", advantage, gpu, _F32, rows)
     if ref_logprob is not None:
-        ref_logprob = _vector("ref_logprob", ref_logprob, device, _F32, x.rows)
+        ref_logprob = _vector("ref_logprob", ref_logprob, gpu, _F32, rows)
     if weight is not None:
-        weight = _vector("weight", weight, device, _F32, x.rows)
+        weight = _vector("weight", weight, gpu, _F32, rows)
     if out is not None and not grad:
         _refuse("out is the gradient's tensor: grad must be True")
-    dz = _grad_like(logits, out) if grad else None
-    p = _Policy(_ptr(old_logprob), _ptr(ref_logprob), _ptr(advantage), _ptr(weight), clip_low, clip_high, kl_coef)
-    res = torch.empty((3, x.rows), dtype=torch.float32, device=device)
-    loss, logprob, kl = res[0], res[1], res[2]
-    clipped = torch.empty(x.rows, dtype=torch.bool, device=device)
-    _check(lib.dlr_policy_loss(device.index, _stream(device), C.byref(x), C.byref(p), loss.data_ptr(),
-                               logprob.data_ptr(), kl.data_ptr(), clipped.data_ptr(), _ptr(dz),
-                               0 if dz is None else dz.stride(0)))
+    dz = _grad_like(logits, out, gpu) if grad else None
+    p = _Policy(old_logprob.data_ptr(), _ptr(ref_logprob), advantage.data_ptr(), _ptr(weight), clip_low, clip_high,
+                kl_coef)
+    (loss, logprob, kl), at = _rows(3, rows, logits)
+    clipped = torch.empty(rows, dtype=torch.bool, device=logits.device)
+    _check(lib.dlr_policy_loss(gpu, _stream(gpu), C.byref(x), C.byref(p), at, at + 4 * rows, at + 8 * rows,
+                               clipped.data_ptr(), _ptr(dz), 0 if dz is None else dz.stride(0)))
     return PolicyLoss(loss, logprob, kl, clipped, dz)
 
 
@@ -223,28 +232,27 @@ def preference_loss(logprob: torch.Tensor, ref_logprob: Optional[torch.Tensor], 
     (average: per counted token); loss = -(1 - label_smoothing) log sigma(u) -
     label_smoothing log sigma(-u), u = chosen_reward - rejected_reward -
     margin.  weight (P) defaults to 1."""
-    device = _gpu("logprob", logprob)
-    tokens = logprob.shape[0] if logprob.dim() == 1 else -1
-    if tokens < 0:
+    gpu = _gpu("logprob", logprob)
+    if logprob.dim() != 1:
         _refuse(f"logprob must have 1 dimension (it has {logprob.dim()})")
-    logprob = _vector("logprob", logprob, device, _F32, tokens)
+    tokens = logprob.shape[0]
+    logprob = _vector("logprob", logprob, gpu, _F32, tokens)
     if ref_logprob is not None:
-        ref_logprob = _vector("ref_logprob", ref_logprob, device, _F32, tokens)
-    if _gpu("offsets", offsets).type == "cuda" and (offsets.dim() != 1 or offsets.shape[0] % 2 != 1):
+        ref_logprob = _vector("ref_logprob", ref_logprob, gpu, _F32, tokens)
+    _gpu("offsets", offsets)
+    if offsets.dim() != 1 or offsets.shape[0] % 2 != 1:
         _refuse("offsets must have 2 P + 1 entries")
     pairs = offsets.shape[0] // 2
-    offsets = _vector("offsets", offsets, device, (torch.int64,), 2 * pairs + 1)
+    offsets = _vector("offsets", offsets, gpu, (torch.int64,), 2 * pairs + 1)
     if mask is not None:
-        mask = _vector("mask", mask, device, _BOOL, tokens)
+        mask = _vector("mask", mask, gpu, _BOOL, tokens)
     if weight is not None:
-        weight = _vector("weight", weight, device, _F32, pairs)
-    p = _Preference(_ptr(logprob), _ptr(ref_logprob), _ptr(mask), _ptr(offsets), _ptr(weight), pairs, tokens, beta,
-                    label_smoothing, margin, 1 if average else 0, 0)
-    res = torch.empty((3, pairs), dtype=torch.float32, device=device)
-    loss, chosen, rejected = res[0], res[1], res[2]
-    dl = torch.empty(tokens, dtype=torch.float32, device=device) if grad else None
-    _check(lib.dlr_preference_loss(device.index, _stream(device), C.byref(p), loss.data_ptr(), chosen.data_ptr(),
-                                   rejected.data_ptr(), _ptr(dl)))
+        weight = _vector("weight", weight, gpu, _F32, pairs)
+    p = _Preference(logprob.data_ptr(), _ptr(ref_logprob), _ptr(mask), offsets.data_ptr(), _ptr(weight), pairs, tokens,
+                    beta, label_smoothing, margin, 1 if average else 0, 0)
+    (loss, chosen, rejected), at = _rows(3, pairs, logprob)
+    dl = torch.empty(tokens, dtype=torch.float32, device=logprob.device) if grad else None
+    _check(lib.dlr_preference_loss(gpu, _stream(gpu), C.byref(p), at, at + 4 * pairs, at + 8 * pairs, _ptr(dl)))
     return PreferenceLoss(loss, chosen, rejected, dl)
 
 
@@ -253,23 +261,19 @@ def head_logprob(hidden: torch.Tensor, head: torch.Tensor, target: torch.Tensor,
     """token_logprob of the logits hidden (rows x dim) . head^T (vocab x dim),
     which are never written out: scoring by a model that is not trained.
     bfloat16 or float16, sums in 32 bits (dlr_head_logprob)."""
-    device = _gpu("hidden", hidden)
-    _matrix("hidden", hidden)
-    if _gpu("head", head) != device:
-        _refuse(f"head is on {head.device}, not on {device}")
-    _matrix("head", head)
+    gpu = _gpu("hidden", hidden)
+    _matrix("hidden", hidden, gpu)
+    _matrix("head", head, gpu)
     if hidden.dtype not in (torch.bfloat16, torch.float16) or head.dtype != hidden.dtype:
         _refuse(f"hidden and head must both be bfloat16 or float16 (they are {hidden.dtype} and {head.dtype})")
     rows, dim = hidden.shape
     if head.shape[1] != dim:
         _refuse(f"hidden has rows of {dim}, head of {head.shape[1]}")
-    target = _vector("target", target, device, _INTS, rows)
+    target = _vector("target", target, gpu, _INTS, rows)
     h = _Head(hidden.data_ptr(), head.data_ptr(), target.data_ptr(), rows, head.shape[0], dim, hidden.stride(0),
               head.stride(0), _DTYPES[hidden.dtype], _TARGET_BITS[target.dtype], temperature)
     need = _check(lib.dlr_head_logprob_workspace(rows, head.shape[0], dim))
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    out = torch.empty((2, rows), dtype=torch.float32, device=device)
-    logprob, lse = out[0], out[1]
-    _check(lib.dlr_head_logprob(device.index, _stream(device), C.byref(h), workspace.data_ptr(), need,
-                                logprob.data_ptr(), lse.data_ptr()))
-    return logprob, lse
+    workspace = torch.empty(need, dtype=torch.uint8, device=hidden.device)
+    out, at = _rows(2, rows, hidden)
+    _check(lib.dlr_head_logprob(gpu, _stream(gpu), C.byref(h), workspace.data_ptr(), need, at, at + 4 * rows))
+    return out
