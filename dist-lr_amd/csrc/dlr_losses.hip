@@ -103,6 +103,20 @@ struct Pack<_Float16> {
     }
 };
 
+// A pack of a row.  `once`: past the caches, for logits that are more than
+// they hold (the flag is the launch's; see kOnceBytes).
+template <typename T>
+__device__ inline u32x4 load_pack(const T *row, int64_t p, bool once) {
+    const u32x4_any *at = reinterpret_cast<const u32x4_any *>(row + p * Pack<T>::N);
+    return once ? __builtin_nontemporal_load(at) : *at;
+}
+// Gradients are written past the caches: 4,096 x 131,072 bf16 467 -> 454 us,
+// 1,021 x 50,257 f32 91 -> 76 us.
+template <typename T>
+__device__ inline void store_pack(T *row, int64_t p, const u32x4 &v) {
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any *>(row + p * Pack<T>::N));
+}
+
 __device__ inline int64_t load_target(const void *target, int bits, int64_t t) {
     return bits == 64 ? static_cast<const int64_t *>(target)[t] : static_cast<const int32_t *>(target)[t];
 }
@@ -178,7 +192,7 @@ __device__ inline float tree_sum(const float (&e)[N]) {
 // One pass over a row: U packs a thread in flight, one rescaling of the
 // running sum per U packs.
 template <typename T, int NT, int U>
-__device__ inline RowStat row_stat(const T *row, int vocab, ExpScale k) {
+__device__ inline RowStat row_stat(const T *row, int vocab, ExpScale k, bool once) {
     using PK = Pack<T>;
     constexpr int N = PK::N;
     const int packs = vocab / N;
@@ -190,7 +204,7 @@ __device__ inline RowStat row_stat(const T *row, int vocab, ExpScale k) {
         for (int u = 0; u < U; ++u) {
             const int p = base + u * NT;
             have[u] = p < packs;
-            if (have[u]) v[u] = *reinterpret_cast<const u32x4_any *>(row + (int64_t)p * N);
+            if (have[u]) v[u] = load_pack(row, p, once);
         }
         float m = a.m;
 #pragma unroll
@@ -232,7 +246,8 @@ __device__ inline double target_logprob(float zy, float m, double ln_s, double t
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t stride, int vocab, const void *target,
-                                                      int target_bits, ExpScale k, double tau, float *logprob, float *lse) {
+                                                      int target_bits, ExpScale k, double tau, bool once, float *logprob,
+                                                      float *lse) {
     __shared__ BlockLds<NT> lds;
     const int64_t t = blockIdx.x;
     const int64_t y = load_target(target, target_bits, t);
@@ -245,7 +260,7 @@ __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t s
     }
     const T *row = logits + t * stride;
     const float zy = y < vocab ? (float)row[y] : __builtin_nanf("");
-    const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
+    const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k, once), k, lds);
     if (threadIdx.x == 0) {
         const double ln = log(a.s);
         lse[t] = (float)(a.m / tau + ln);
@@ -259,7 +274,7 @@ __device__ inline void zero_row(T *out, int vocab) {
     constexpr int N = Pack<T>::N;
     const int packs = vocab / N;
     const u32x4 z = {0u, 0u, 0u, 0u};
-    for (int p = threadIdx.x; p < packs; p += NT) *reinterpret_cast<u32x4_any *>(out + (int64_t)p * N) = z;
+    for (int p = threadIdx.x; p < packs; p += NT) store_pack(out, p, z);
     const int tail = packs * N + threadIdx.x;
     if (tail < vocab) out[tail] = (T)0.f;
 }
@@ -268,7 +283,7 @@ __device__ inline void zero_row(T *out, int vocab) {
 // exponent's two forms chosen by the caller (see the kernels).  Each thread
 // reads a pack before it writes it, so out may be the row itself.
 template <typename T, int NT, int U, typename F>
-__device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, float c, F prob) {
+__device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, float c, F prob, bool once) {
     using PK = Pack<T>;
     constexpr int N = PK::N;
     const int packs = vocab / N;
@@ -277,7 +292,7 @@ __device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int p = base + u * NT;
-            if (p < packs) v[u] = *reinterpret_cast<const u32x4_any *>(row + (int64_t)p * N);
+            if (p < packs) v[u] = load_pack(row, p, once);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -291,7 +306,7 @@ __device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, 
 #pragma unroll
                 for (int i = 0; i < N; ++i) f[i] += i == at ? c : 0.f;
             }
-            *reinterpret_cast<u32x4_any *>(out + (int64_t)p * N) = PK::put(f);
+            store_pack(out, p, PK::put(f));
         }
     }
     const int tail = packs * N + threadIdx.x;
@@ -305,7 +320,7 @@ constexpr float kLseExact = 128.f;
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int64_t stride, int vocab,
-                                                           const void *target, int target_bits, double tau,
+                                                           const void *target, int target_bits, double tau, bool once,
                                                            const float *lse, const float *grad, T *out,
                                                            int64_t out_stride) {
     const int64_t t = blockIdx.x;
@@ -321,15 +336,15 @@ __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int6
     if (fabsf(l) > kLseExact) {
         __shared__ BlockLds<NT> lds;
         const ExpScale k = exp_scale(tau);
-        const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(logits + t * stride, vocab, k), k, lds);
+        const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(logits + t * stride, vocab, k, false), k, lds);
         const float neg = (float)(-c / a.s), m = a.m;
         residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
-                               [=](float z) { return neg * exp2_hw((z - m) * k.hi); });
+                               [=](float z) { return neg * exp2_hw((z - m) * k.hi); }, once);
         return;
     }
     const float it = (float)(1.0 / tau);
     residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
-                           [=](float z) { return -c * exp2_hw(__builtin_fmaf(z, it, -l) * 1.44269504f); });
+                           [=](float z) { return -c * exp2_hw(__builtin_fmaf(z, it, -l) * 1.44269504f); }, once);
 }
 
 // ---------------------------------------------------------------- policy loss
@@ -368,10 +383,76 @@ __device__ inline double policy_token(double lp, const dlr_policy &p, int64_t t,
     return slope * w;
 }
 
-template <typename T, int NT>
+// A row held in registers: R packs a thread, pack i of thread x at i NT + x,
+// and the element of the tail that is this thread's.
+template <typename T, int NT, int R>
+struct HeldRow {
+    using PK = Pack<T>;
+    u32x4 v[R];
+    float tail;
+
+    __device__ void load(const T *row, int vocab, bool once) {
+        const int packs = vocab / PK::N;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int p = i * NT + threadIdx.x;
+            if (p < packs) v[i] = load_pack(row, p, once);
+        }
+        const int at = packs * PK::N + threadIdx.x;
+        tail = at < vocab ? (float)row[at] : NEG_INF;
+    }
+    __device__ RowStat stat(int vocab, ExpScale k) const {
+        const int packs = vocab / PK::N;
+        float m = tail;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i * NT + (int)threadIdx.x < packs) {
+#pragma unroll
+                for (int e = 0; e < PK::N; ++e) m = fmaxf(m, PK::get(v[i], e));
+            }
+        const float r = m == NEG_INF ? 0.f : m;
+        float s[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            s[i] = 0.f;
+            if (i * NT + (int)threadIdx.x < packs) {
+                float x[PK::N];
+#pragma unroll
+                for (int e = 0; e < PK::N; ++e) x[e] = exp2_scaled(PK::get(v[i], e) - r, k);
+                s[i] = tree_sum(x);
+            }
+        }
+        return {m, tree_sum(s) + exp2_scaled(tail - r, k)};
+    }
+    template <typename F>
+    __device__ void residual(T *out, int vocab, int64_t y, float c, F prob) const {
+        const int packs = vocab / PK::N;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int p = i * NT + threadIdx.x;
+            if (p >= packs) continue;
+            float f[PK::N];
+#pragma unroll
+            for (int e = 0; e < PK::N; ++e) f[e] = prob(PK::get(v[i], e));
+            const int64_t at = y - (int64_t)p * PK::N;
+            if (at >= 0 && at < PK::N) {
+#pragma unroll
+                for (int e = 0; e < PK::N; ++e) f[e] += e == at ? c : 0.f;
+            }
+            store_pack(out, p, PK::put(f));
+        }
+        const int at = packs * PK::N + threadIdx.x;
+        if (at < vocab) out[at] = (T)(prob(tail) + (at == y ? c : 0.f));
+    }
+};
+
+// Logits to gradient with one read: a row's coefficient needs the whole row's
+// statistics, so the row stays in registers until they are known.  REST: rows
+// longer than R NT packs; what does not fit is read again.
+template <typename T, int NT, int R, bool REST>
 __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t stride, int vocab, const void *target,
-                                                    int target_bits, ExpScale k, double tau, dlr_policy p, PolicyOut po,
-                                                    T *out, int64_t out_stride) {
+                                                    int target_bits, ExpScale k, double tau, bool once, dlr_policy p,
+                                                    PolicyOut po, T *out, int64_t out_stride) {
     __shared__ BlockLds<NT> lds;
     __shared__ float coef;
     const int64_t t = blockIdx.x;
@@ -385,9 +466,15 @@ __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t str
         if (out) zero_row<T, NT>(out + t * out_stride, vocab);
         return;
     }
+    constexpr int kHeld = R * NT * Pack<T>::N;
+    const int here = REST ? kHeld : vocab;
     const T *row = logits + t * stride;
+    HeldRow<T, NT, R> held;
+    held.load(row, here, once);
     const float zy = y < vocab ? (float)row[y] : __builtin_nanf("");
-    const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k), k, lds);
+    RowStat own = held.stat(here, k);
+    if constexpr (REST) own = join(own, row_stat<T, NT, 4>(row + kHeld, vocab - kHeld, k, false), k);
+    const BlockStat a = join_block<NT>(own, k, lds);
     if (threadIdx.x == 0) {
         const double lp = target_logprob(zy, a.m, log(a.s), tau);
         coef = (float)(policy_token(lp, p, t, w, po) / tau);
@@ -395,8 +482,10 @@ __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t str
     if (!out) return;
     __syncthreads();
     const float c = coef, neg = (float)(-c / a.s), m = a.m;
-    residual_row<T, NT, 4>(row, out + t * out_stride, vocab, y, c,
-                           [=](float z) { return neg * exp2_hw((z - m) * k.hi); });
+    auto prob = [=](float z) { return neg * exp2_hw((z - m) * k.hi); };
+    T *o = out + t * out_stride;
+    held.residual(o, here, y, c, prob);
+    if constexpr (REST) residual_row<T, NT, 4>(row + kHeld, o + kHeld, vocab - kHeld, y - kHeld, c, prob, once);
 }
 
 // ------------------------------------------------------------ preference loss
@@ -875,12 +964,19 @@ static hipError_t by_dtype(int dtype, F f) {
     return hipGetLastError();
 }
 
+// Logits of more bytes than the 256 MB Infinity Cache cannot be there when the
+// call begins, nor will a second read find them: they are read past it.
+constexpr int64_t kOnceBytes = INT64_C(1) << 28;
+static bool read_once(const dlr_logits &x) {
+    return x.rows * x.vocab * (x.dtype == DLR_DTYPE_F32 ? 4 : 2) > kOnceBytes;
+}
+
 hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
         k_token_logprob<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
             static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
-            x.temperature, logprob, lse);
+            x.temperature, read_once(x), logprob, lse);
     });
 }
 
@@ -889,18 +985,37 @@ hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const 
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
         k_token_logprob_grad<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
-            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, x.temperature, lse,
-            grad, static_cast<T *>(out), out_stride);
+            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, x.temperature,
+            read_once(x), lse, grad, static_cast<T *>(out), out_stride);
     });
+}
+
+template <typename T, int NT, int R, bool REST = false>
+static void launch_policy(hipStream_t st, const dlr_logits &x, const dlr_policy &p, const PolicyOut &po, void *out,
+                          int64_t out_stride) {
+    k_policy_loss<T, NT, R, REST><<<dim3((unsigned)x.rows), NT, 0, st>>>(
+        static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
+        x.temperature, read_once(x), p, po, static_cast<T *>(out), out_stride);
 }
 
 hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, float *loss, float *logprob,
                               float *kl, uint8_t *clipped, void *out, int64_t out_stride) {
+    const PolicyOut po{loss, logprob, kl, clipped};
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
-        k_policy_loss<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
-            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
-            x.temperature, p, PolicyOut{loss, logprob, kl, clipped}, static_cast<T *>(out), out_stride);
+        const int64_t packs = x.vocab / Pack<T>::N;
+        if (packs <= 512)
+            launch_policy<T, 128, 4>(st, x, p, po, out, out_stride);
+        else if (packs <= 1024)
+            launch_policy<T, 256, 4>(st, x, p, po, out, out_stride);
+        else if (packs <= 4096)
+            launch_policy<T, 512, 8>(st, x, p, po, out, out_stride);
+        else if (packs <= 8192)
+            launch_policy<T, 512, 16>(st, x, p, po, out, out_stride);
+        else if (packs <= 16384)
+            launch_policy<T, 1024, 16>(st, x, p, po, out, out_stride);
+        else
+            launch_policy<T, 1024, sizeof(T) == 4 ? 16 : 8, true>(st, x, p, po, out, out_stride);
     });
 }
 
