@@ -971,22 +971,55 @@ static bool read_once(const dlr_logits &x) {
     return x.rows * x.vocab * (x.dtype == DLR_DTYPE_F32 ? 4 : 2) > kOnceBytes;
 }
 
+// A row's threads.  Short rows: as few as keep a few packs each, for the
+// rows' ends (joining, the logarithm) are what costs (8,000 x 1,000 bf16: 7.8
+// us with 64 threads, 20 with 512).  Long rows: enough loads in flight
+// (1 x 32,000: 4.9 us with 512, 12.8 with 64; 4,096 x 131,072: 189 against
+// 195).
+template <typename T, int NT>
+static void launch_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
+    k_token_logprob<T, NT><<<dim3((unsigned)x.rows), NT, 0, st>>>(
+        static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
+        x.temperature, read_once(x), logprob, lse);
+}
+
 hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
-        k_token_logprob<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
-            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
-            x.temperature, read_once(x), logprob, lse);
+        const int64_t packs = x.vocab / Pack<T>::N;
+        if (packs <= 256)
+            launch_logprob<T, 64>(st, x, logprob, lse);
+        else if (packs <= 1024)
+            launch_logprob<T, 128>(st, x, logprob, lse);
+        else
+            launch_logprob<T, 512>(st, x, logprob, lse);
     });
 }
 
+template <typename T, int NT>
+static void launch_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad, void *out,
+                        int64_t out_stride) {
+    k_token_logprob_grad<T, NT><<<dim3((unsigned)x.rows), NT, 0, st>>>(
+        static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, x.temperature,
+        read_once(x), lse, grad, static_cast<T *>(out), out_stride);
+}
+
+// As above; rows of 2,048 to 16,384 packs gain from fewer of them in flight
+// at once (8,192 x 32,000 bf16 191 -> 174 us with 1,024 threads a row), longer
+// ones lose (4,096 x 131,072 f32 810 -> 864).
 hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad,
                                      void *out, int64_t out_stride) {
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
-        k_token_logprob_grad<T, 512><<<dim3((unsigned)x.rows), 512, 0, st>>>(
-            static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, x.temperature,
-            read_once(x), lse, grad, static_cast<T *>(out), out_stride);
+        const int64_t packs = x.vocab / Pack<T>::N;
+        if (packs <= 256)
+            launch_grad<T, 64>(st, x, lse, grad, out, out_stride);
+        else if (packs <= 1024)
+            launch_grad<T, 128>(st, x, lse, grad, out, out_stride);
+        else if (packs <= 2048 || packs > 16384)
+            launch_grad<T, 512>(st, x, lse, grad, out, out_stride);
+        else
+            launch_grad<T, 1024>(st, x, lse, grad, out, out_stride);
     });
 }
 
