@@ -721,6 +721,41 @@ __device__ inline void lds_dma16(const void *src, void *lds) {
                                      (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
 }
 
+// The rows that take part, in order, where they are picked first (row not
+// null): row[0 .. *count).
+struct HeadPick {
+    const int32_t *row;
+    const int64_t *count;
+};
+
+// Picks them, one workgroup; the others' results are written here.
+__global__ __launch_bounds__(1024) void k_head_pick(const void *target, int target_bits, int64_t rows, int32_t *row,
+                                                    int64_t *count, float *logprob, float *lse) {
+    __shared__ int found[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t total = 0;
+    for (int64_t base = 0; base < rows; base += 1024) {
+        const int64_t t = base + threadIdx.x;
+        const bool on = t < rows && load_target(target, target_bits, t) >= 0;
+        const uint64_t mask = __ballot(on);
+        if (lane == 0) found[wave] = __popcll(mask);
+        __syncthreads();
+        int64_t at = total + __popcll(mask & ((UINT64_C(1) << lane) - 1));
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) at += found[w];
+            total += found[w];
+        }
+        if (on) {
+            row[at] = (int32_t)t;
+        } else if (t < rows) {
+            logprob[t] = 0.f;
+            lse[t] = 0.f;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *count = total;
+}
+
 // One scheduling group: N instructions of a kind (8: MFMA, 32: memory reads,
 // 256: LDS reads), in program order with the groups around it.
 #define SCHED_MFMA(n) __builtin_amdgcn_sched_group_barrier(8, n, 0)
@@ -728,23 +763,25 @@ __device__ inline void lds_dma16(const void *src, void *lds) {
 #define SCHED_LDS(n) __builtin_amdgcn_sched_group_barrier(256, n, 0)
 
 template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
-__global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int vtiles, int ttiles, float2 *part,
-                                                               float *zy) {
+__global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, HeadPick pick, float2 *part, float *zy) {
     constexpr int NW = WV * WT, TV = WV * MV * 16, TT = WT * MT * 16, kRow = 128;
     constexpr int kLoads = (TV + TT) / 8, L = (kLoads + NW - 1) / NW;  // DMA loads of 8 rows: all, a wave's
     static_assert(TV % 8 == 0 && TT % 8 == 0 && S >= 2 && L * (S - 2) < 64, "whole loads, a wait that can be written");
     __shared__ __attribute__((aligned(256))) char sm[S][(TV + TT) * kRow];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wv = wave / WT, wt = wave % WT;
+    const int64_t used = pick.row ? *pick.count : h.rows;
+    const int64_t vtiles = (h.vocab + TV - 1) / TV, ttiles = (used + TT - 1) / TT;
     // XCD x takes a contiguous piece of the tile order, in which up to 8
     // token tiles of one class tile follow each other: an XCD's 32 running
     // workgroups share 8 token and 4 class tiles in its L2.
     int64_t tile = blockIdx.x;
     {
-        const int64_t n = (int64_t)vtiles * ttiles, q = n / 8, rem = n % 8, x = tile % 8;
+        const int64_t n = vtiles * ttiles, q = n / 8, rem = n % 8, x = tile % 8;
+        if (tile >= n) return;  // the launch counts all rows
         tile = x * q + (x < rem ? x : rem) + tile / 8;
     }
-    const int64_t group = (int64_t)vtiles * 8;  // tiles of 8 token tiles' group
+    const int64_t group = vtiles * 8;  // tiles of 8 token tiles' group
     const int64_t g = tile / group;
     const int in_g = ttiles - g * 8 < 8 ? (int)(ttiles - g * 8) : 8;
     const int64_t rest = tile - g * group;
@@ -756,7 +793,9 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int v
     // Rows outside repeat the last one; a wave without an L-th load repeats
     // the last load (every wave then has L of them in flight per stage).
     const char *base_v = static_cast<const char *>(h.head) + v0 * h.head_stride * 2;
-    const char *base_t = static_cast<const char *>(h.hidden) + t0 * h.hidden_stride * 2;
+    const int64_t t_base = pick.row ? 0 : t0;
+    const char *base_t = static_cast<const char *>(h.hidden) + t_base * h.hidden_stride * 2;
+    auto token = [&](int64_t t) { return pick.row ? (int64_t)pick.row[t] : t; };
     uint32_t off[L];
     const int chunk = (lane & 7) ^ (lane >> 3);
     auto load_no = [&](int q) {
@@ -768,8 +807,9 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int v
         const int n = load_no(q);
         const bool x = n >= TV / 8;
         const int r = (x ? n - TV / 8 : n) * 8 + (lane >> 3);
-        const int64_t last = x ? h.rows - 1 - t0 : h.vocab - 1 - v0;
-        off[q] = (uint32_t)((r < last ? r : last) * (x ? h.hidden_stride : h.head_stride) * 2 + chunk * 16);
+        const int64_t last = x ? used - 1 - t0 : h.vocab - 1 - v0;
+        const int64_t at = r < last ? r : last;
+        off[q] = (uint32_t)((x ? (token(t0 + at) - t_base) * h.hidden_stride : at * h.head_stride) * 2 + chunk * 16);
     }
     auto fill = [&](int step, int buf) {
         const char *sv = base_v + (int64_t)step * 128, *st = base_t + (int64_t)step * 128;
@@ -866,7 +906,8 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int v
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
         const int64_t t = t0 + wt * MT * 16 + j * 16 + (lane & 15);
-        const int64_t y = t < h.rows ? load_target(h.target, h.target_bits, t) : -1;
+        const int64_t row = t < used ? token(t) : -1;
+        const int64_t y = row >= 0 ? load_target(h.target, h.target_bits, row) : -1;
         const int64_t base = v0 + wv * MV * 16 + (lane >> 4) * 4;
         float m = NEG_INF;
 #pragma unroll
@@ -874,7 +915,7 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int v
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (ragged && base + i * 16 + e >= h.vocab) acc[i][j][e] = NEG_INF;
-                if (base + i * 16 + e == y) zy[t] = acc[i][j][e];
+                if (base + i * 16 + e == y) zy[row] = acc[i][j][e];
                 m = fmaxf(m, acc[i][j][e]);
             }
         m = fmaxf(m, __shfl_xor(m, 16));
@@ -895,7 +936,7 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int v
     }
     __syncthreads();
     for (int i = tid; i < TT; i += NW * 64)
-        if (t0 + i < h.rows) {
+        if (t0 + i < used) {
             RowStat a = stat[i];
 #pragma unroll
             for (int w = 1; w < WV; ++w) a = join(a, stat[w * TT + i], k);
@@ -907,23 +948,26 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int v
 // side by side), 256 / RT threads each.  The maximum first, then the scaled
 // sums in 64 bits (as join_block); a thread keeps its first 16 tiles.
 template <int RT>
-__global__ __launch_bounds__(256) void k_head_join(dlr_head h, int64_t tiles, const float2 *part, const float *zy,
-                                                   float *logprob, float *lse) {
+__global__ __launch_bounds__(256) void k_head_join(dlr_head h, HeadPick pick, int64_t tiles, const float2 *part,
+                                                   const float *zy, float *logprob, float *lse) {
     constexpr int G = 256 / RT, K = 16;
     __shared__ float lm[4][RT];
     __shared__ double ls[4][RT];
     const int tok = threadIdx.x % RT, first = threadIdx.x / RT, wave = threadIdx.x >> 6;
-    const int64_t t = (int64_t)blockIdx.x * RT + tok;
-    const int64_t y = t < h.rows ? load_target(h.target, h.target_bits, t) : -1;
+    const int64_t t = (int64_t)blockIdx.x * RT + tok, used = pick.row ? *pick.count : h.rows;
+    const bool in = t < used;
+    const int64_t row = !in ? 0 : pick.row ? (int64_t)pick.row[t] : t;
+    const int64_t y = in ? load_target(h.target, h.target_bits, row) : -1;
     const ExpScale k = exp_scale(h.temperature);
-    const float2 *p = part + (t < h.rows ? t : 0);
+    const float2 *p = part + (in ? t : 0);
+    if (!in) tiles = 0;
     float2 q[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) {
         const int64_t n = first + i * G;
         q[i] = n < tiles ? p[n * h.rows] : make_float2(NEG_INF, 0.f);
     }
-    const float z = y >= 0 && y < h.vocab ? zy[t] : __builtin_nanf("");
+    const float z = y >= 0 && y < h.vocab ? zy[row] : __builtin_nanf("");
     float m = NEG_INF;
 #pragma unroll
     for (int i = 0; i < K; ++i) m = fmaxf(m, q[i].x);
@@ -945,11 +989,11 @@ __global__ __launch_bounds__(256) void k_head_join(dlr_head h, int64_t tiles, co
     for (int o = RT; o < 64; o <<= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) < RT) ls[wave][tok] = s;
     __syncthreads();
-    if (first || t >= h.rows) return;
+    if (first || !in) return;
     s = (ls[0][tok] + ls[1][tok]) + (ls[2][tok] + ls[3][tok]);
     const double tau = h.temperature, ln = log(s);
-    lse[t] = y < 0 ? 0.f : (float)(m / tau + ln);
-    logprob[t] = y < 0 ? 0.f : (float)target_logprob(z, m, ln, tau);
+    lse[row] = y < 0 ? 0.f : (float)(m / tau + ln);
+    logprob[row] = y < 0 ? 0.f : (float)target_logprob(z, m, ln, tau);
 }
 
 }  // namespace
@@ -1074,18 +1118,41 @@ static bool head_by_dma(const dlr_head &h) {
 
 constexpr int kSmallestTile = 64;  // classes: the most tiles, for the workspace
 
+// The workspace: the targets' logits, the picked rows and their count, the
+// tiles' statistics.
+struct HeadSpace {
+    float *zy;
+    int32_t *row;
+    int64_t *count;
+    float2 *part;
+};
+static int64_t head_part(int64_t rows) { return (rows * 8 + 8 + 255) / 256 * 256; }  // where the statistics begin
+
 int64_t head_workspace(int64_t rows, int64_t vocab) {
     const int64_t tiles = (vocab + kSmallestTile - 1) / kSmallestTile;
-    return rows * tiles * (int64_t)sizeof(float2) + (rows + 1) / 2 * 2 * (int64_t)sizeof(float);
+    return head_part(rows) + rows * tiles * (int64_t)sizeof(float2);
+}
+
+static HeadSpace head_space(void *workspace, int64_t rows) {
+    char *w = static_cast<char *>(workspace);
+    return {reinterpret_cast<float *>(w + 8), reinterpret_cast<int32_t *>(w + 8 + rows * 4),
+            reinterpret_cast<int64_t *>(w), reinterpret_cast<float2 *>(w + head_part(rows))};
+}
+
+// Whether the rows that take part are picked first, so that the others cost
+// nothing: 4 us for what may be half of a long call, from about 100 us on.
+static bool head_picks(const dlr_head &h) {
+    return (double)h.rows * (double)h.vocab * (double)h.dim >= 6.4e10 && h.rows > 64 &&
+           h.rows * h.hidden_stride < (INT64_C(1) << 31);  // 32-bit places of any row
 }
 
 template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
-static int64_t launch_head_dma(hipStream_t st, const dlr_head &h, float2 *part, float *zy) {
+static int64_t launch_head_dma(hipStream_t st, const dlr_head &h, const HeadPick &pick, const HeadSpace &w) {
     constexpr int TV = WV * MV * 16, TT = WT * MT * 16;
     static_assert(TV >= kSmallestTile, "the workspace counts on it");
     const int64_t vtiles = (h.vocab + TV - 1) / TV, ttiles = (h.rows + TT - 1) / TT;
-    k_head_dma<T, WV, WT, MV, MT, S, OCC><<<dim3((unsigned)(vtiles * ttiles)), WV * WT * 64, 0, st>>>(
-        h, (int)vtiles, (int)ttiles, part, zy);
+    k_head_dma<T, WV, WT, MV, MT, S, OCC><<<dim3((unsigned)(vtiles * ttiles)), WV * WT * 64, 0, st>>>(h, pick,
+                                                                                                           w.part, w.zy);
     return vtiles;
 }
 
@@ -1099,39 +1166,44 @@ static int64_t launch_head_dma(hipStream_t st, const dlr_head &h, float2 *part, 
 // 4096 x 32000: 63 us by 256 x 128, 95 by 256 x 256; 2048 x 4096 x 1000: 30
 // us by 128 x 64, 81).
 template <typename T>
-static int64_t launch_head_tiles(hipStream_t st, const dlr_head &h, float2 *part, float *zy) {
+static int64_t launch_head_tiles(hipStream_t st, const dlr_head &h, const HeadPick &pick, const HeadSpace &w) {
     if (!head_by_dma(h)) {
         const int64_t vtiles = (h.vocab + kTileV - 1) / kTileV;
-        k_head_tile<T><<<dim3((unsigned)(vtiles * ((h.rows + kTileT - 1) / kTileT))), 256, 0, st>>>(h, part, zy);
+        k_head_tile<T><<<dim3((unsigned)(vtiles * ((h.rows + kTileT - 1) / kTileT))), 256, 0, st>>>(h, w.part, w.zy);
         return vtiles;
     }
     constexpr int64_t kCus = 256;
     if (h.rows <= 16)
-        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, part, zy)
-                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, part, zy);
+        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, pick, w)
+                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, pick, w);
     auto tiles = [&](int64_t tv, int64_t tt) { return ((h.vocab + tv - 1) / tv) * ((h.rows + tt - 1) / tt); };
     auto rounds = [&](int64_t n, int64_t slots) { return (double)((n + slots - 1) / slots); };
     auto pair = [&](int64_t n, double alone, double two) { return n <= kCus ? alone : two * rounds(n, 2 * kCus); };
     const double a = rounds(tiles(256, 256), kCus), b = 0.6 * rounds(tiles(256, 128), kCus),
                  c = pair(tiles(128, 64), 0.35, 0.41), d = pair(tiles(64, 64), 0.27, 0.4);
-    if (a <= b && a <= c && a <= d) return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, part, zy);
-    if (b <= c && b <= d) return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, part, zy);
-    if (c <= d) return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, part, zy);
-    return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, part, zy);
+    if (a <= b && a <= c && a <= d) return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, pick, w);
+    if (b <= c && b <= d) return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, pick, w);
+    if (c <= d) return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, pick, w);
+    return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, pick, w);
 }
 
 hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
-    // zy first: its place does not depend on the kernel's tiles
-    float *zy = static_cast<float *>(workspace);
-    float2 *part = reinterpret_cast<float2 *>(zy + (h.rows + 1) / 2 * 2);
-    const int64_t tiles = h.dtype == DLR_DTYPE_BF16 ? launch_head_tiles<__bf16>(st, h, part, zy)
-                                                    : launch_head_tiles<_Float16>(st, h, part, zy);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    const HeadSpace w = head_space(workspace, h.rows);
+    const bool picks = head_by_dma(h) && head_picks(h);
+    const HeadPick pick{picks ? w.row : nullptr, w.count};
+    hipError_t e;
+    if (picks) {
+        k_head_pick<<<1, 1024, 0, st>>>(h.target, h.target_bits, h.rows, w.row, w.count, logprob, lse);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    const int64_t tiles = h.dtype == DLR_DTYPE_BF16 ? launch_head_tiles<__bf16>(st, h, pick, w)
+                                                    : launch_head_tiles<_Float16>(st, h, pick, w);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
     if (h.rows < 16)
-        k_head_join<1><<<dim3((unsigned)h.rows), 256, 0, st>>>(h, tiles, part, zy, logprob, lse);
+        k_head_join<1><<<dim3((unsigned)h.rows), 256, 0, st>>>(h, pick, tiles, w.part, w.zy, logprob, lse);
     else
-        k_head_join<16><<<dim3((unsigned)((h.rows + 15) / 16)), 256, 0, st>>>(h, tiles, part, zy, logprob, lse);
+        k_head_join<16><<<dim3((unsigned)((h.rows + 15) / 16)), 256, 0, st>>>(h, pick, tiles, w.part, w.zy, logprob,
+                                                                               lse);
     return hipGetLastError();
 }
 

@@ -650,3 +650,30 @@ def test_refusals_on_the_gpu(L, dlr):
     assert lp.shape == (0,)
     assert L.token_logprob_grad(z[:0], y[:0], v[:0], v[:0]).shape == (0, 5)
     assert L.policy_loss(z[:0], y[:0], v[:0], v[:0]).grad.shape == (0, 5)
+
+
+@pytest.mark.parametrize("out", ["none", "half", "all", "all but the last", "all but the first 130"])
+def test_head_long_calls_leave_out_the_rows_that_take_no_part(L, out):
+    # from rows * vocab * dim = 6.4e10 on the rows that take part are picked first
+    rows, vocab, dim = 700, 50001, 2048
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    x = torch.randint(-2, 3, (rows, dim), generator=g, device="cuda").bfloat16()
+    w = torch.randint(-2, 3, (vocab, dim), generator=g, device="cuda").bfloat16()
+    y = make_target(rows, vocab)
+    keep = torch.ones(rows, dtype=torch.bool)
+    if out == "half":
+        keep = torch.rand(rows, generator=gen(4)) < 0.5
+    elif out != "none":
+        keep[:] = False
+        keep[-1] = out == "all but the last"
+        keep[:130] = out == "all but the first 130"
+    y[~keep] = -7
+    x[~keep.cuda()] = float("nan")
+    scale = 60.0
+    lp, lse = L.head_logprob(x, w, y.cuda(), temperature=scale)
+    z = torch.mm(torch.nan_to_num(x).double(), w.double().t()).cpu()  # whole numbers: exact
+    want_lp, want_lse = ref_logprob(z, y, scale)
+    e = lse_tol(vocab) + U * 3 * 12
+    close(lse, want_lse, torch.where(keep, e + U * want_lse.abs(), 0.0))
+    close(lp, want_lp, torch.where(keep, e + U * want_lp.abs(), 0.0))
