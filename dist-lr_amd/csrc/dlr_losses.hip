@@ -793,9 +793,10 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, HeadP
     // Rows outside repeat the last one; a wave without an L-th load repeats
     // the last load (every wave then has L of them in flight per stage).
     const char *base_v = static_cast<const char *>(h.head) + v0 * h.head_stride * 2;
-    const int64_t t_base = pick.row ? 0 : t0;
+    const bool picked = pick.row && used < h.rows;  // all of them: in their places, without a trip to the list
+    const int64_t t_base = picked ? 0 : t0;
     const char *base_t = static_cast<const char *>(h.hidden) + t_base * h.hidden_stride * 2;
-    auto token = [&](int64_t t) { return pick.row ? (int64_t)pick.row[t] : t; };
+    auto token = [&](int64_t t) { return picked ? (int64_t)pick.row[t] : t; };
     uint32_t off[L];
     const int chunk = (lane & 7) ^ (lane >> 3);
     auto load_no = [&](int q) {
