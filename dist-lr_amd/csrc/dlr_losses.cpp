@@ -2,18 +2,18 @@
 // host can see is checked here, before anything is enqueued.
 #include "dlr_losses.h"
 
-#include <cmath>
-#include <string>
+#include <dlfcn.h>
 
-#include "dlr_internal.h"
+#include <cmath>
+#include <cstdio>
+#include <initializer_list>
 
 namespace {
 
+thread_local char last_error[512] = "";
+
 int refuse(int code, const char *call, const char *why) noexcept {
-    try {
-        dlr::set_error(std::string(call) + ": " + why);
-    } catch (...) {  // no memory for the message: the code still says it
-    }
+    (void)std::snprintf(last_error, sizeof last_error, "%s: %s", call, why);
     return code;
 }
 
@@ -109,6 +109,13 @@ bool floats(std::initializer_list<const void *> ps) {
 }  // namespace
 
 extern "C" {
+
+const char *dlr_losses_last_error(void) { return last_error; }
+
+const char *dlr_losses_runtime(void) {
+    Dl_info info;
+    return dladdr(reinterpret_cast<const void *>(&hipGetDevice), &info) && info.dli_fname ? info.dli_fname : "";
+}
 
 int dlr_token_logprob(int device, void *stream, const dlr_logits *x, float *logprob, float *lse) {
     const char *call = "dlr_token_logprob";

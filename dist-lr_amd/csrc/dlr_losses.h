@@ -7,7 +7,7 @@
 
 #include <cstdint>
 
-#include "distlr_amd.h"
+#include "distlr_losses.h"
 
 namespace dlr {
 

@@ -59,8 +59,6 @@ SYMBOLS = [
     "dlr_timing", "dlr_kernel_time", "dlr_stage_time", "dlr_stage_counters", "dlr_train_layout", "dlr_train_band_rows", "dlr_train_relabeled", "dlr_train_unit_values", "dlr_train_product_margin", "dlr_train_pm_strided", "dlr_train_hot_columns", "dlr_train_row_rounds",
     "dlr_set_exchange_overlap", "dlr_exchange_overlap", "dlr_set_exchange_pieces", "dlr_exchange_pieces",
     "dlr_memory_info", "dlr_stream_bytes",
-    "dlr_token_logprob", "dlr_token_logprob_grad", "dlr_policy_loss", "dlr_preference_loss",
-    "dlr_head_logprob_workspace", "dlr_head_logprob",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -228,12 +226,6 @@ _sig("dlr_set_exchange_pieces", C.c_int, P, C.c_int)
 _sig("dlr_exchange_pieces", C.c_int, P)
 _sig("dlr_memory_info", C.c_int, P, C.POINTER(i64), C.POINTER(i64))
 _sig("dlr_stream_bytes", C.c_int, P, C.POINTER(i64), C.POINTER(i64))
-_sig("dlr_token_logprob", C.c_int, C.c_int, P, P, P, P)
-_sig("dlr_token_logprob_grad", C.c_int, C.c_int, P, P, P, P, P, i64)
-_sig("dlr_policy_loss", C.c_int, C.c_int, P, P, P, P, P, P, P, P, i64)
-_sig("dlr_preference_loss", C.c_int, C.c_int, P, P, P, P, P, P)
-_sig("dlr_head_logprob_workspace", i64, i64, i64, i64)
-_sig("dlr_head_logprob", C.c_int, C.c_int, P, P, P, i64, P, P)
 
 
 class DLRError(RuntimeError):

@@ -1,5 +1,4 @@
-"""Softmax losses on torch tensors (the device section of
-include/distlr_amd.h): log-probabilities of given classes and their gradient,
+"""Softmax losses on torch tensors (include/distlr_losses.h): log-probabilities of given classes and their gradient,
 the paired logistic (preference) loss, the clipped policy loss, and
 log-probabilities straight from hidden states and the output layer's weights.
 
@@ -12,35 +11,52 @@ GPU and may be captured into a graph; results and scratch memory come from
 torch's allocator.  As with torch's own operators, a tensor made on another
 stream has to be waited for by the caller.  Arguments that do not fit raise
 ``DLRError`` with code ``E_ARG`` before anything is enqueued.
-
-Import torch before this package, so that the process has one HIP runtime.
 """
 from __future__ import annotations
 
 import ctypes as C
+import os
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import E_ARG, DLRError, _check, lib
+from . import E_ARG, PKG, DLRError
+
+LIB_PATH = os.path.join(PKG, "lib", "libdistlr_losses.so")
+LIB_PATH = os.environ.get("DLR_LOSSES_LIB", LIB_PATH)  # as DLR_LIB: a variant build of the same library
+
+if not os.path.exists(LIB_PATH):
+    raise ImportError(f"{LIB_PATH} not built: run `make -C dist-lr_amd` (or __graft_entry__.build())")
+
+lib = C.CDLL(LIB_PATH)  # after torch: it takes the runtime torch has loaded
+
+P, i64 = C.c_void_p, C.c_int64
+SYMBOLS = {
+    "dlr_losses_last_error": (C.c_char_p,),
+    "dlr_losses_runtime": (C.c_char_p,),
+    "dlr_token_logprob": (C.c_int, C.c_int, P, P, P, P),
+    "dlr_token_logprob_grad": (C.c_int, C.c_int, P, P, P, P, P, i64),
+    "dlr_policy_loss": (C.c_int, C.c_int, P, P, P, P, P, P, P, P, i64),
+    "dlr_preference_loss": (C.c_int, C.c_int, P, P, P, P, P, P),
+    "dlr_head_logprob_workspace": (i64, i64, i64, i64),
+    "dlr_head_logprob": (C.c_int, C.c_int, P, P, P, i64, P, P),
+}
+for _name, (_res, *_args) in SYMBOLS.items():
+    getattr(lib, _name).restype, getattr(lib, _name).argtypes = _res, _args
+
+_runtime = os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so")  # where torch brings its own
+if os.path.exists(_runtime) and not os.path.samefile(lib.dlr_losses_runtime().decode(), _runtime):
+    raise ImportError(f"{LIB_PATH} is bound to {lib.dlr_losses_runtime().decode()}, not to torch's HIP runtime")
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 _DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 _TARGET_BITS = {torch.int32: 32, torch.int64: 64}
 
 
-def _one_runtime() -> None:
-    """A stream of one HIP runtime means nothing to another one."""
-    try:
-        with open("/proc/self/maps") as f:
-            seen = {line.split()[-1] for line in f if "/libamdhip64.so" in line}
-    except OSError:
-        return
-    if len(seen) > 1:
-        raise ImportError(f"two HIP runtimes in this process ({', '.join(sorted(seen))}): import torch before distlr_amd")
-
-
-_one_runtime()
+def _check(rc: int) -> int:
+    if rc < 0:
+        raise DLRError(rc, lib.dlr_losses_last_error().decode(errors="replace"))
+    return rc
 
 
 class _Logits(C.Structure):

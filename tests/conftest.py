@@ -12,11 +12,6 @@ import sys
 
 import pytest
 
-try:  # before any test imports distlr_amd: the process then has one HIP runtime, torch's, which
-    import torch  # noqa: F401  distlr_amd.losses needs (bench.py and smoke() import in this order too)
-except ImportError:
-    pass
-
 ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 GOLDEN = os.path.join(ROOT, "tests", "golden")
 sys.path.insert(0, os.path.join(ROOT, "dist-lr_amd"))

@@ -22,7 +22,7 @@ import math
 
 import pytest
 
-torch = pytest.importorskip("torch")  # before distlr_amd: one HIP runtime
+torch = pytest.importorskip("torch")
 
 pytestmark = pytest.mark.gpu
 

@@ -6,10 +6,12 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 
-torch = pytest.importorskip("torch")  # before distlr_amd: one HIP runtime
+torch = pytest.importorskip("torch")
 
 import distlr_amd as dlr  # noqa: E402
 import distlr_amd.losses as L  # noqa: E402
@@ -20,9 +22,34 @@ BASE = (C.addressof(BUF) + 255) // 256 * 256
 A, B, D, E, F = (BASE + 8192 * i for i in range(5))
 
 
+HEADER = os.path.join(ROOT, "include", "distlr_losses.h")
+
+
+def test_header_library_and_binding_agree():
+    with open(HEADER) as f:
+        text = re.sub(r"/\*.*?\*/", "", f.read(), flags=re.S)
+    declared = sorted(set(re.findall(r"\b(dlr_[a-z0-9_]+)\s*\(", text)))
+    out = subprocess.run(["nm", "-D", "--defined-only", L.LIB_PATH], check=True, capture_output=True, text=True).stdout
+    exported = {line.split()[-1] for line in out.splitlines() if line.strip()}
+    assert sorted(L.SYMBOLS) == declared and set(declared) <= exported
+    with open(L.LIB_PATH, "rb") as f:
+        assert b"amdgcn-amd-amdhsa--gfx950" in f.read()
+
+
+@pytest.mark.parametrize("order", ["torch, distlr_amd.losses", "distlr_amd, torch, distlr_amd.losses",
+                                   "distlr_amd.losses"])
+def test_the_library_takes_torchs_runtime_in_any_order_of_imports(order):
+    prog = (f"import sys; sys.path.insert(0, {os.path.join(ROOT, 'dist-lr_amd')!r})\n"
+            f"import {order}\nimport torch, distlr_amd.losses as L, os\n"
+            "own = os.path.join(os.path.dirname(torch.__file__), 'lib', 'libamdhip64.so')\n"
+            "print(not os.path.exists(own) or os.path.samefile(L.lib.dlr_losses_runtime().decode(), own))")
+    out = subprocess.run([sys.executable, "-c", prog], check=True, capture_output=True, text=True).stdout
+    assert out.strip() == "True"
+
+
 def code(rc):
     assert rc < 0
-    return rc, dlr.lib.dlr_last_error(None).decode()
+    return rc, L.lib.dlr_losses_last_error().decode()
 
 
 def logits(**kw):
@@ -45,9 +72,9 @@ BAD_LOGITS = [
 @pytest.mark.parametrize("kw,word", BAD_LOGITS, ids=lambda v: str(v)[:40])
 def test_bad_logits_are_refused_by_every_call(kw, word):
     x, p = logits(**kw), L._Policy(D, None, D, None, 0.2, 0.2, 0.0)
-    for rc in (dlr.lib.dlr_token_logprob(0, None, C.byref(x), D, E),
-               dlr.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, D, E, 8),
-               dlr.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, E, None, 0)):
+    for rc in (L.lib.dlr_token_logprob(0, None, C.byref(x), D, E),
+               L.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, D, E, 8),
+               L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, E, None, 0)):
         rc, msg = code(rc)
         assert rc == dlr.E_ARG and word in msg
 
@@ -55,18 +82,18 @@ def test_bad_logits_are_refused_by_every_call(kw, word):
 def test_null_descriptors_and_outputs():
     x, p = logits(), L._Policy(D, None, D, None, 0.2, 0.2, 0.0)
     calls = [
-        lambda: dlr.lib.dlr_token_logprob(0, None, None, D, E),
-        lambda: dlr.lib.dlr_token_logprob(0, None, C.byref(x), None, E),
-        lambda: dlr.lib.dlr_token_logprob(0, None, C.byref(x), D, None),
-        lambda: dlr.lib.dlr_token_logprob(0, None, C.byref(x), D + 2, E),
-        lambda: dlr.lib.dlr_token_logprob_grad(0, None, C.byref(x), None, D, E, 8),
-        lambda: dlr.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, None, E, 8),
-        lambda: dlr.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, D, None, 8),
-        lambda: dlr.lib.dlr_policy_loss(0, None, C.byref(x), None, E, E, E, E, None, 0),
-        lambda: dlr.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, E, E, E, None, 0),
-        lambda: dlr.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, None, None, 0),
-        lambda: dlr.lib.dlr_preference_loss(0, None, None, E, E, E, None),
-        lambda: dlr.lib.dlr_head_logprob(0, None, None, D, 1 << 20, E, E),
+        lambda: L.lib.dlr_token_logprob(0, None, None, D, E),
+        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), None, E),
+        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), D, None),
+        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), D + 2, E),
+        lambda: L.lib.dlr_token_logprob_grad(0, None, C.byref(x), None, D, E, 8),
+        lambda: L.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, None, E, 8),
+        lambda: L.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, D, None, 8),
+        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), None, E, E, E, E, None, 0),
+        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, E, E, E, None, 0),
+        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, None, None, 0),
+        lambda: L.lib.dlr_preference_loss(0, None, None, E, E, E, None),
+        lambda: L.lib.dlr_head_logprob(0, None, None, D, 1 << 20, E, E),
     ]
     for call in calls:
         assert code(call())[0] == dlr.E_ARG
@@ -77,15 +104,15 @@ def test_null_descriptors_and_outputs():
     (A, 9, "overlap"), (A + 4 * 31, 8, "overlap"), (A - 4, 8, "overlap")])
 def test_gradients_that_do_not_fit(grad, stride, word):
     x, p = logits(), L._Policy(E, None, E, None, 0.2, 0.2, 0.0)
-    for rc in (dlr.lib.dlr_token_logprob_grad(0, None, C.byref(x), E, E, grad, stride),
-               dlr.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), F, F, F, F, grad, stride)):
+    for rc in (L.lib.dlr_token_logprob_grad(0, None, C.byref(x), E, E, grad, stride),
+               L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), F, F, F, F, grad, stride)):
         rc, msg = code(rc)
         assert rc == dlr.E_ARG and word in msg
 
 
 def test_gradient_over_logits_whose_rows_share_memory():
     x = logits(row_stride=0)
-    rc, msg = code(dlr.lib.dlr_token_logprob_grad(0, None, C.byref(x), E, E, A, 0))
+    rc, msg = code(L.lib.dlr_token_logprob_grad(0, None, C.byref(x), E, E, A, 0))
     assert rc == dlr.E_ARG
 
 
@@ -98,7 +125,7 @@ def test_bad_policy(kw, word):
     v = dict(old_logprob=D, ref_logprob=D, advantage=D, weight=None, clip_low=0.2, clip_high=0.2, kl_coef=0.1)
     v.update(kw)
     x, p = logits(), L._Policy(**v)
-    rc, msg = code(dlr.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, E, None, 0))
+    rc, msg = code(L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, E, None, 0))
     assert rc == dlr.E_ARG and word in msg
 
 
@@ -113,13 +140,13 @@ def test_bad_preference(kw, word):
              label_smoothing=0.0, margin=0.0, average=0, reserved=0)
     v.update(kw)
     p = L._Preference(**v)
-    rc, msg = code(dlr.lib.dlr_preference_loss(0, None, C.byref(p), D, D, D, E))
+    rc, msg = code(L.lib.dlr_preference_loss(0, None, C.byref(p), D, D, D, E))
     assert rc == dlr.E_ARG and word in msg
 
 
 def test_preference_gradient_over_an_input():
     p = L._Preference(A, None, None, B, None, 2, 10, 0.1, 0.0, 0.0, 0, 0)
-    rc, msg = code(dlr.lib.dlr_preference_loss(0, None, C.byref(p), D, D, D, A + 8))
+    rc, msg = code(L.lib.dlr_preference_loss(0, None, C.byref(p), D, D, D, A + 8))
     assert rc == dlr.E_ARG and "overlap" in msg
 
 
@@ -134,35 +161,35 @@ def test_bad_head(kw, word):
              dtype=L.DTYPE_BF16, target_bits=64, temperature=1.0)
     v.update(kw)
     h = L._Head(**v)
-    rc, msg = code(dlr.lib.dlr_head_logprob(0, None, C.byref(h), D, 1 << 30, E, E))
+    rc, msg = code(L.lib.dlr_head_logprob(0, None, C.byref(h), D, 1 << 30, E, E))
     assert rc == dlr.E_ARG and word in msg
 
 
 def test_head_workspace():
-    need = dlr.lib.dlr_head_logprob_workspace(4, 100, 64)
+    need = L.lib.dlr_head_logprob_workspace(4, 100, 64)
     assert need > 0
-    assert code(dlr.lib.dlr_head_logprob_workspace(4, 0, 64))[0] == dlr.E_ARG
+    assert code(L.lib.dlr_head_logprob_workspace(4, 0, 64))[0] == dlr.E_ARG
     h = L._Head(A, A, B, 4, 100, 64, 64, 64, L.DTYPE_BF16, 64, 1.0)
     for ws, size in ((None, need), (D, need - 1), (D + 4, need)):
-        rc, msg = code(dlr.lib.dlr_head_logprob(0, None, C.byref(h), ws, size, E, E))
+        rc, msg = code(L.lib.dlr_head_logprob(0, None, C.byref(h), ws, size, E, E))
         assert rc == dlr.E_ARG and "workspace" in msg
 
 
 def test_no_rows_is_a_valid_call():
     x, p = logits(rows=0, data=None, target=None), L._Policy(None, None, None, None, 0.2, 0.2, 0.0)
-    assert dlr.lib.dlr_token_logprob(0, None, C.byref(x), None, None) == 0
-    assert dlr.lib.dlr_token_logprob_grad(0, None, C.byref(x), None, None, None, 0) == 0
-    assert dlr.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, None, None, None, None, 0) == 0
+    assert L.lib.dlr_token_logprob(0, None, C.byref(x), None, None) == 0
+    assert L.lib.dlr_token_logprob_grad(0, None, C.byref(x), None, None, None, 0) == 0
+    assert L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, None, None, None, None, 0) == 0
     q = L._Preference(None, None, None, None, None, 0, 0, 0.1, 0.0, 0.0, 0, 0)
-    assert dlr.lib.dlr_preference_loss(0, None, C.byref(q), None, None, None, None) == 0
+    assert L.lib.dlr_preference_loss(0, None, C.byref(q), None, None, None, None) == 0
     h = L._Head(None, None, None, 0, 100, 64, 64, 64, L.DTYPE_BF16, 64, 1.0)
-    assert dlr.lib.dlr_head_logprob(0, None, C.byref(h), None, 0, None, None) == 0
+    assert L.lib.dlr_head_logprob(0, None, C.byref(h), None, 0, None, None) == 0
 
 
 @pytest.mark.parametrize("struct,name", [(L._Logits, "dlr_logits"), (L._Policy, "dlr_policy"),
                                          (L._Preference, "dlr_preference"), (L._Head, "dlr_head")])
 def test_structs_match_the_header(struct, name):
-    with open(os.path.join(ROOT, "include", "distlr_amd.h")) as f:
+    with open(HEADER) as f:
         text = re.sub(r"/\*.*?\*/", "", f.read(), flags=re.S)
     body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
     ctype = {"const void *": C.c_void_p, "const float *": C.c_void_p, "const uint8_t *": C.c_void_p,
