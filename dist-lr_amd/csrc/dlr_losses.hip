@@ -707,6 +707,7 @@ __global__ __launch_bounds__(256) void k_head_tile(dlr_head h, float2 *part, flo
 
 // ---- aligned rows: both operands through LDS by DMA
 //
+// Classes v_first .. h.vocab - 1, `part` from the first of their tiles on.
 // A workgroup of WV x WT waves takes TV = WV * 16 * MV classes x TT = WT * 16
 // * MT tokens, 64 of the dimension (a stage) at a time, S stages in LDS.
 // Rows of a stage are 128 bytes, classes first; the 16-byte chunk c of row r
@@ -763,7 +764,8 @@ __global__ __launch_bounds__(1024) void k_head_pick(const void *target, int targ
 #define SCHED_LDS(n) __builtin_amdgcn_sched_group_barrier(256, n, 0)
 
 template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
-__global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, HeadPick pick, float2 *part, float *zy) {
+__global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int64_t v_first, HeadPick pick, float2 *part,
+                                                               float *zy) {
     constexpr int NW = WV * WT, TV = WV * MV * 16, TT = WT * MT * 16, kRow = 128;
     constexpr int kLoads = (TV + TT) / 8, L = (kLoads + NW - 1) / NW;  // DMA loads of 8 rows: all, a wave's
     static_assert(TV % 8 == 0 && TT % 8 == 0 && S >= 2 && L * (S - 2) < 64, "whole loads, a wait that can be written");
@@ -771,7 +773,7 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, HeadP
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wv = wave / WT, wt = wave % WT;
     const int64_t used = pick.row ? *pick.count : h.rows;
-    const int64_t vtiles = (h.vocab + TV - 1) / TV, ttiles = (used + TT - 1) / TT;
+    const int64_t vtiles = (h.vocab - v_first + TV - 1) / TV, ttiles = (used + TT - 1) / TT;
     // XCD x takes a contiguous piece of the tile order, in which up to 8
     // token tiles of one class tile follow each other: an XCD's 32 running
     // workgroups share 8 token and 4 class tiles in its L2.
@@ -786,7 +788,7 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, HeadP
     const int in_g = ttiles - g * 8 < 8 ? (int)(ttiles - g * 8) : 8;
     const int64_t rest = tile - g * group;
     const int64_t vt = rest / in_g, tt = g * 8 + rest % in_g;
-    const int64_t v0 = vt * TV, t0 = tt * TT;
+    const int64_t v0 = v_first + vt * TV, t0 = tt * TT;
     const int dim = (int)h.dim, full = dim / 64, steps = (dim + 63) / 64;
 
     // This lane's places in the wave's DMA loads, from the tile's first row.
@@ -1147,25 +1149,75 @@ static bool head_picks(const dlr_head &h) {
            h.rows * h.hidden_stride < (INT64_C(1) << 31);  // 32-bit places of any row
 }
 
+// Classes [first, end); tile0: the statistics' first tile.  Returns the next.
 template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
-static int64_t launch_head_dma(hipStream_t st, const dlr_head &h, const HeadPick &pick, const HeadSpace &w) {
+static int64_t launch_head_dma(hipStream_t st, dlr_head h, int64_t first, int64_t end, const HeadPick &pick,
+                               const HeadSpace &w, int64_t tile0) {
     constexpr int TV = WV * MV * 16, TT = WT * MT * 16;
     static_assert(TV >= kSmallestTile, "the workspace counts on it");
-    const int64_t vtiles = (h.vocab + TV - 1) / TV, ttiles = (h.rows + TT - 1) / TT;
-    k_head_dma<T, WV, WT, MV, MT, S, OCC><<<dim3((unsigned)(vtiles * ttiles)), WV * WT * 64, 0, st>>>(h, pick,
-                                                                                                           w.part, w.zy);
-    return vtiles;
+    const int64_t vtiles = (end - first + TV - 1) / TV, ttiles = (h.rows + TT - 1) / TT;
+    h.vocab = end;
+    k_head_dma<T, WV, WT, MV, MT, S, OCC><<<dim3((unsigned)(vtiles * ttiles)), WV * WT * 64, 0, st>>>(
+        h, first, pick, w.part + tile0 * h.rows, w.zy);
+    return tile0 + vtiles;
 }
 
-// The tile.  Up to 16 rows the head's bytes are all there is: 256 classes a
-// workgroup once that is two workgroups a CU, else 64 with a deeper queue
-// (1 row x 4096: 131,072 classes 180 us against 190, 65,536 classes 105
-// against 118).  Beyond, the cheapest by rounds of the 256 CUs, in units of a
-// 256 x 256 tile's time (80 us at dim 4096; the others' as measured there
-// alone on a CU and two on one): 256 x 256 runs at 1,360 TFLOP/s full, 256 x
-// 128 at 1,195, and the small ones fill the CUs where those cannot (200 x
-// 4096 x 32000: 63 us by 256 x 128, 95 by 256 x 256; 2048 x 4096 x 1000: 30
-// us by 128 x 64, 81).
+// The tiles of more than 16 rows.  What a tile costs: microseconds per stage
+// of 64, alone on its CU or two of them on it, measured from 1 x 8 to 32,768
+// tiles at dim 512 and 4096; and per round of the CUs its ends.
+struct HeadTile {
+    int64_t tv, tt;
+    double alone, two;  // two 0: one workgroup a CU
+};
+constexpr HeadTile kHeadTiles[] = {{256, 256, 1.56, 0}, {256, 128, 0.9, 0}, {128, 64, 0.42, 0.67}, {64, 64, 0.3, 0.55}};
+constexpr int64_t kCus = 256;
+constexpr double kEnds = 3, kLaunch = 3;
+
+static double head_cost(const HeadTile &t, int64_t rows, int64_t classes, int64_t stages) {
+    if (classes <= 0) return 0;
+    const int64_t n = ((classes + t.tv - 1) / t.tv) * ((rows + t.tt - 1) / t.tt);
+    if (t.two == 0 || n <= kCus) return (double)((n + kCus - 1) / kCus) * (t.alone * stages + kEnds);
+    return (double)((n + 2 * kCus - 1) / (2 * kCus)) * (t.two * stages + kEnds);
+}
+
+// A plan: the first `classes` by tile `first`, the others by tile `rest`.
+struct HeadPlan {
+    int first, rest;
+    int64_t classes;
+};
+
+// The cheapest tile for all classes, or a large one for as many classes as
+// fill whole rounds of the CUs and the cheapest for the others: 333 x 1536 x
+// 50257 is 2.3 rounds of 256 x 128 tiles, paid as 3 (74 us), or one round of
+// 256 x 256 tiles and one of 256 x 128.
+static HeadPlan head_plan(const dlr_head &h) {
+    const int64_t stages = (h.dim + 63) / 64;
+    auto best = [&](int64_t classes) {
+        int i = 0;
+        for (int j = 1; j < 4; ++j)
+            if (head_cost(kHeadTiles[j], h.rows, classes, stages) < head_cost(kHeadTiles[i], h.rows, classes, stages))
+                i = j;
+        return i;
+    };
+    const int whole = best(h.vocab);
+    HeadPlan plan{whole, whole, h.vocab};
+    double cost = head_cost(kHeadTiles[whole], h.rows, h.vocab, stages);
+    for (int i = 0; i < 2; ++i) {
+        const HeadTile &t = kHeadTiles[i];
+        const int64_t ttiles = (h.rows + t.tt - 1) / t.tt, rounds = h.vocab / t.tv * ttiles / kCus;
+        const int64_t classes = rounds * kCus / ttiles * t.tv;
+        if (classes <= 0 || classes >= h.vocab) continue;
+        const int rest = best(h.vocab - classes);
+        const double c = head_cost(t, h.rows, classes, stages) + kLaunch +
+                         head_cost(kHeadTiles[rest], h.rows, h.vocab - classes, stages);
+        if (c < cost) {
+            plan = {i, rest, classes};
+            cost = c;
+        }
+    }
+    return plan;
+}
+
 template <typename T>
 static int64_t launch_head_tiles(hipStream_t st, const dlr_head &h, const HeadPick &pick, const HeadSpace &w) {
     if (!head_by_dma(h)) {
@@ -1173,19 +1225,25 @@ static int64_t launch_head_tiles(hipStream_t st, const dlr_head &h, const HeadPi
         k_head_tile<T><<<dim3((unsigned)(vtiles * ((h.rows + kTileT - 1) / kTileT))), 256, 0, st>>>(h, w.part, w.zy);
         return vtiles;
     }
-    constexpr int64_t kCus = 256;
+    // Up to 16 rows the head's bytes are all there is: 256 classes a workgroup
+    // once that is most of two workgroups a CU, else 64 with a deeper queue (1
+    // row x 4096: 131,072 classes 180 us against 190, 65,536 classes 118
+    // against 105).
     if (h.rows <= 16)
-        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, pick, w)
-                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, pick, w);
-    auto tiles = [&](int64_t tv, int64_t tt) { return ((h.vocab + tv - 1) / tv) * ((h.rows + tt - 1) / tt); };
-    auto rounds = [&](int64_t n, int64_t slots) { return (double)((n + slots - 1) / slots); };
-    auto pair = [&](int64_t n, double alone, double two) { return n <= kCus ? alone : two * rounds(n, 2 * kCus); };
-    const double a = rounds(tiles(256, 256), kCus), b = 0.6 * rounds(tiles(256, 128), kCus),
-                 c = pair(tiles(128, 64), 0.35, 0.41), d = pair(tiles(64, 64), 0.27, 0.4);
-    if (a <= b && a <= c && a <= d) return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, pick, w);
-    if (b <= c && b <= d) return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, pick, w);
-    if (c <= d) return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, pick, w);
-    return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, pick, w);
+        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, 0, h.vocab, pick, w, 0)
+                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, 0, h.vocab, pick, w, 0);
+    auto launch = [&](int tile, int64_t first, int64_t end, int64_t tile0) {
+        switch (tile) {
+            case 0: return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, first, end, pick, w, tile0);
+            case 1: return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, first, end, pick, w, tile0);
+            case 2: return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, first, end, pick, w, tile0);
+            default: return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, first, end, pick, w, tile0);
+        }
+    };
+    const HeadPlan plan = head_plan(h);
+    int64_t tiles = launch(plan.first, 0, plan.classes, 0);
+    if (plan.classes < h.vocab) tiles = launch(plan.rest, plan.classes, h.vocab, tiles);
+    return tiles;
 }
 
 hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
