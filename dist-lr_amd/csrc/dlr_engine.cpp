@@ -53,7 +53,6 @@ struct StreamArr {
     std::vector<int64_t> beg, end;
     std::shared_ptr<void> keep;  // the host array, page-locked
     const char *host = nullptr;
-    bool registered = false;
     void *slot[2] = {nullptr, nullptr};
     size_t cap = 0;  // elements per slot
 };
@@ -176,7 +175,7 @@ struct TrainShard {
     uint32_t dref_seq = 0;
     int dref_lead = 0;
     // streamed dense shard (DLR_RESIDENCY_STREAM): X stays in the caller's
-    // host memory (registered, pinned in place); each batch's rows and labels
+    // host memory (registered where the driver allows it); each batch's rows and labels
     // are staged into one of two device slots on the copy stream
     bool streamed = false, host_registered = false;
     const float *hX = nullptr;
@@ -570,7 +569,6 @@ void free_train(dlr_ctx *c) {
     if (t.sparse_stream) {
         if (c->cstream) (void)hipStreamSynchronize(c->cstream);
         for (StreamArr &a : t.sarr) {
-            if (a.registered) (void)hipHostUnregister(const_cast<char *>(a.host));
             dev_free(c, a.slot[0]);
             dev_free(c, a.slot[1]);
             *a.field = nullptr;  // the bound view pointed into a slot
@@ -622,16 +620,13 @@ int place(dlr_ctx *c, T **field, const T *src, size_t n, size_t pad, const Range
         a.end[(size_t)b] = std::max(r.first, r.second);
         if (a.end[(size_t)b] > a.beg[(size_t)b]) cap = std::max(cap, (size_t)(a.end[(size_t)b] - a.beg[(size_t)b]) + pad);
     }
-    auto *hv = new std::vector<T>(n + pad);  // zero tail: the padded reads of the last batch
-    if (n) std::copy(src, src + n, hv->begin());
-    a.keep = std::shared_ptr<void>(hv, [](void *p) { delete static_cast<std::vector<T> *>(p); });
-    a.host = reinterpret_cast<const char *>(hv->data());
-    hipError_t e = hipHostRegister(const_cast<char *>(a.host), (n + pad) * sizeof(T), hipHostRegisterDefault);
-    if (e != hipSuccess) {
-        (void)hipGetLastError();
-        return fail(c, DLR_E_HIP, std::string("dlr_load_train: hipHostRegister (streamed shard): ") + hipGetErrorString(e));
-    }
-    a.registered = true;
+    // page-locked by its allocation: a driver may refuse to lock memory that exists
+    T *hv = nullptr;
+    HIPC(c, hipHostMalloc((void **)&hv, std::max<size_t>(n + pad, 1) * sizeof(T), hipHostMallocDefault));
+    a.keep = std::shared_ptr<void>(hv, [](void *p) { (void)hipHostFree(p); });
+    if (n) std::copy(src, src + n, hv);
+    std::fill(hv + n, hv + n + pad, T());  // zero tail: the padded reads of the last batch
+    a.host = reinterpret_cast<const char *>(hv);
     a.cap = cap;
     *field = nullptr;
     t.sarr.push_back(std::move(a));
@@ -1495,8 +1490,6 @@ int coalesce_stream(dlr_ctx *c, int nthreads) {
         }
     });
     for (StreamArr &a : t.sarr) {  // the array-major copies and slots are no longer needed
-        if (a.registered) (void)hipHostUnregister(const_cast<char *>(a.host));
-        a.registered = false;
         a.keep.reset();
         a.host = nullptr;
         for (int k = 0; k < 2; ++k) {
@@ -3598,12 +3591,10 @@ int dlr_load_train_dense(dlr_ctx *c, const dlr_dense *ds, int64_t batch_size, in
         t.streamed = true;
         t.hX = ds->X.data();
         hipError_t e = hipHostRegister(const_cast<float *>(t.hX), xbytes, hipHostRegisterDefault);
-        if (e == hipSuccess)
-            t.host_registered = true;
-        else if (e == hipErrorHostMemoryAlreadyRegistered)
-            (void)hipGetLastError();
-        else
-            return fail(c, DLR_E_HIP, std::string("dlr_load_train_dense: hipHostRegister: ") + hipGetErrorString(e));
+        // refused (or registered already): the rows are copied as they are,
+        // through the driver's own staging where they are pageable
+        t.host_registered = e == hipSuccess;
+        if (e != hipSuccess) (void)hipGetLastError();
         if (!c->cstream) HIPC(c, hipStreamCreateWithFlags(&c->cstream, hipStreamNonBlocking));
         for (int k = 0; k < 2; ++k) {
             if (!c->ev_ready[k]) HIPC(c, hipEventCreateWithFlags(&c->ev_ready[k], hipEventDisableTiming));

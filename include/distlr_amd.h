@@ -293,7 +293,8 @@ int dlr_load_test_dense(dlr_ctx *ctx, const dlr_dense *ds);
  * 328 GB, more than one GPU's HBM).  DEVICE uploads the shard once; STREAM
  * keeps it in page-locked host memory and copies each batch into one of two
  * device slots on a copy stream while the previous batch computes --
- * PCIe-bound.  Dense shards stream the caller's rows in place (registered:
+ * PCIe-bound.  Dense shards stream the caller's rows in place (page-locked
+ * where the driver allows that of existing memory, else as they are, slower:
  * the dlr_dense must outlive the loaded shard); sparse shards stream a
  * page-locked, batch-major copy of their CSR and per-batch column-major
  * slices, each batch staged by ONE copy (every
