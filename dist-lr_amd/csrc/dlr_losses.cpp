@@ -27,6 +27,7 @@ class DeviceScope {
         if (err_ == hipSuccess && before_ != device) {
             err_ = hipSetDevice(device);
             set_ = err_ == hipSuccess;
+            if (!set_) (void)hipGetLastError();  // reported here, not by the caller's next call
         }
     }
     ~DeviceScope() {
@@ -66,7 +67,6 @@ const char *check_target(const void *target, int32_t bits, double temperature) {
     if (!target) return "target is NULL";
     if (bits != 32 && bits != 64) return "target_bits must be 32 or 64";
     if (!aligned(target, bits / 8)) return "target is not aligned to its type";
-    if (!(temperature > 0.0) || !std::isfinite(temperature)) return "temperature must be positive and finite";
     if (!(temperature >= 1e-6 && temperature <= 1e6)) return "temperature must lie in [1e-6, 1e6]";
     return nullptr;
 }

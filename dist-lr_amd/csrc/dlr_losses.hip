@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <tuple>
 
 #include "dlr_losses.h"
 
@@ -244,6 +245,9 @@ __device__ inline double target_logprob(float zy, float m, double ln_s, double t
 
 // ----------------------------------------------------- token log-probabilities
 
+// One row a workgroup, one read.  Bound by memory: 4,096 x 131,072 bf16, a
+// quarter of the rows out, 141 us, 5.7 TB/s of what is read (the exponentials
+// alone would take 55 us); short and few rows by the row's ends.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t stride, int vocab, const void *target,
                                                       int target_bits, ExpScale k, double tau, bool once, float *logprob,
@@ -279,9 +283,9 @@ __device__ inline void zero_row(T *out, int vocab) {
     if (tail < vocab) out[tail] = (T)0.f;
 }
 
-// out_j = (j = y ? c : 0) + neg * 2^(z_j a + b): the softmax residual, the
-// exponent's two forms chosen by the caller (see the kernels).  Each thread
-// reads a pack before it writes it, so out may be the row itself.
+// out_j = (j = y ? c : 0) + prob(z_j), prob the probability times -c: the
+// softmax residual.  Each thread reads a pack before it writes it, so out may
+// be the row itself.
 template <typename T, int NT, int U, typename F>
 __device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, float c, F prob, bool once) {
     using PK = Pack<T>;
@@ -318,6 +322,8 @@ __device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, 
 // with the type's lowest value) take their statistics again.
 constexpr float kLseExact = 128.f;
 
+// One row a workgroup, one read and one write.  Bound by memory: 4,096 x
+// 131,072 bf16 379 us (5.7 TB/s), 2,048 x 50,257 f16 with odd rows 71 us (5.1).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int64_t stride, int vocab,
                                                            const void *target, int target_bits, double tau, bool once,
@@ -369,7 +375,7 @@ __device__ inline double policy_token(double lp, const dlr_policy &p, int64_t t,
     if (p.ref_logprob) {
         const double gap = (double)p.ref_logprob[t] - lp;
         const double e = expm1(gap);
-        kl = e - gap;
+        kl = e - (e == __builtin_inf() ? 0.0 : gap);  // a class of probability 0: inf, not inf - inf
         if (p.kl_coef != 0.0) {
             loss += p.kl_coef * kl;
             slope -= p.kl_coef * e;
@@ -449,6 +455,11 @@ struct HeldRow {
 // Logits to gradient with one read: a row's coefficient needs the whole row's
 // statistics, so the row stays in registers until they are known.  REST: rows
 // longer than R NT packs; what does not fit is read again.
+// Bound by memory: 4,096 x 131,072 bf16 442 us (4.9 TB/s; reading the row a
+// second time instead of holding it 547), 1,021 x 50,257 f32 85 us.  A row of
+// 256 KB fills a CU's registers, so the exponentials of its two passes (17 us
+// of its 27) overlap only with other CUs' memory.  Loading the next row into
+// the registers that the gradient frees spilled them (882 us) and was left out.
 template <typename T, int NT, int R, bool REST>
 __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t stride, int vocab, const void *target,
                                                     int target_bits, ExpScale k, double tau, bool once, dlr_policy p,
@@ -504,7 +515,11 @@ typedef uint32_t u32_any __attribute__((aligned(1)));
 // in 64 bits (they nearly cancel), the logistic loss of their difference, and
 // the pair's one slope written over its tokens.  4 tokens a thread and step,
 // loaded whether the mask counts them or not: a load that waits for its mask
-// costs a second trip to memory (1,024 pairs of 1.5M tokens: 19.6 us so).
+// costs a second trip to memory.  Bound by latency, three dependent trips and
+// the logarithms: 1,024 pairs of 1.5M tokens 9 us (19.6 a token at a time
+// behind its mask), two pairs 4.  One workgroup a pair also where the
+// sequences are very long (1 x 400,000 tokens 69 us): the logits of such a
+// pair take a thousand times as long.
 template <int NT>
 __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOut o) {
     constexpr int H = NT / 2, W = NT / 64;
@@ -1001,14 +1016,29 @@ __global__ __launch_bounds__(256) void k_head_join(dlr_head h, HeadPick pick, in
 
 }  // namespace
 
+// A launch's own error: the runtime's last error may be an earlier call's.
+template <typename... P, typename... A>
+static hipError_t launch(void (*kernel)(P...), int64_t blocks, int threads, hipStream_t st, const A &...a) {
+    static_assert(sizeof...(P) == sizeof...(A), "every argument");
+    std::tuple<P...> values(static_cast<P>(a)...);
+    return std::apply(
+        [&](auto &...v) {
+            void *args[] = {const_cast<void *>(static_cast<const void *>(&v))...};
+            const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3((unsigned)blocks),
+                                                 dim3((unsigned)threads), args, 0, st);
+            if (e != hipSuccess) (void)hipGetLastError();  // reported here, not by the caller's next call
+            return e;
+        },
+        values);
+}
+
 template <typename F>
 static hipError_t by_dtype(int dtype, F f) {
     switch (dtype) {
-        case DLR_DTYPE_F32: f(float()); break;
-        case DLR_DTYPE_BF16: f(__bf16()); break;
-        default: f(_Float16()); break;
+        case DLR_DTYPE_F32: return f(float());
+        case DLR_DTYPE_BF16: return f(__bf16());
+        default: return f(_Float16());
     }
-    return hipGetLastError();
 }
 
 // Logits of more bytes than the 256 MB Infinity Cache cannot be there when the
@@ -1024,31 +1054,27 @@ static bool read_once(const dlr_logits &x) {
 // (1 x 32,000: 4.9 us with 512, 12.8 with 64; 4,096 x 131,072: 189 against
 // 195).
 template <typename T, int NT>
-static void launch_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
-    k_token_logprob<T, NT><<<dim3((unsigned)x.rows), NT, 0, st>>>(
-        static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
-        x.temperature, read_once(x), logprob, lse);
+static hipError_t launch_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
+    return launch(k_token_logprob<T, NT>, x.rows, NT, st, static_cast<const T *>(x.data), x.row_stride, (int)x.vocab,
+                  x.target, x.target_bits, exp_scale(x.temperature), x.temperature, read_once(x), logprob, lse);
 }
 
 hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
         const int64_t packs = x.vocab / Pack<T>::N;
-        if (packs <= 256)
-            launch_logprob<T, 64>(st, x, logprob, lse);
-        else if (packs <= 1024)
-            launch_logprob<T, 128>(st, x, logprob, lse);
-        else
-            launch_logprob<T, 512>(st, x, logprob, lse);
+        if (packs <= 256) return launch_logprob<T, 64>(st, x, logprob, lse);
+        if (packs <= 1024) return launch_logprob<T, 128>(st, x, logprob, lse);
+        return launch_logprob<T, 512>(st, x, logprob, lse);
     });
 }
 
 template <typename T, int NT>
-static void launch_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad, void *out,
-                        int64_t out_stride) {
-    k_token_logprob_grad<T, NT><<<dim3((unsigned)x.rows), NT, 0, st>>>(
-        static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, x.temperature,
-        read_once(x), lse, grad, static_cast<T *>(out), out_stride);
+static hipError_t launch_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad, void *out,
+                              int64_t out_stride) {
+    return launch(k_token_logprob_grad<T, NT>, x.rows, NT, st, static_cast<const T *>(x.data), x.row_stride,
+                  (int)x.vocab, x.target, x.target_bits, x.temperature, read_once(x), lse, grad,
+                  static_cast<T *>(out), out_stride);
 }
 
 // As above; rows of 2,048 to 16,384 packs gain from fewer of them in flight
@@ -1059,23 +1085,19 @@ hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const 
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
         const int64_t packs = x.vocab / Pack<T>::N;
-        if (packs <= 256)
-            launch_grad<T, 64>(st, x, lse, grad, out, out_stride);
-        else if (packs <= 1024)
-            launch_grad<T, 128>(st, x, lse, grad, out, out_stride);
-        else if (packs <= 2048 || packs > 16384)
-            launch_grad<T, 512>(st, x, lse, grad, out, out_stride);
-        else
-            launch_grad<T, 1024>(st, x, lse, grad, out, out_stride);
+        if (packs <= 256) return launch_grad<T, 64>(st, x, lse, grad, out, out_stride);
+        if (packs <= 1024) return launch_grad<T, 128>(st, x, lse, grad, out, out_stride);
+        if (packs <= 2048 || packs > 16384) return launch_grad<T, 512>(st, x, lse, grad, out, out_stride);
+        return launch_grad<T, 1024>(st, x, lse, grad, out, out_stride);
     });
 }
 
 template <typename T, int NT, int R, bool REST = false>
-static void launch_policy(hipStream_t st, const dlr_logits &x, const dlr_policy &p, const PolicyOut &po, void *out,
-                          int64_t out_stride) {
-    k_policy_loss<T, NT, R, REST><<<dim3((unsigned)x.rows), NT, 0, st>>>(
-        static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature),
-        x.temperature, read_once(x), p, po, static_cast<T *>(out), out_stride);
+static hipError_t launch_policy(hipStream_t st, const dlr_logits &x, const dlr_policy &p, const PolicyOut &po,
+                                void *out, int64_t out_stride) {
+    return launch(k_policy_loss<T, NT, R, REST>, x.rows, NT, st, static_cast<const T *>(x.data), x.row_stride,
+                  (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature), x.temperature, read_once(x), p, po,
+                  static_cast<T *>(out), out_stride);
 }
 
 hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, float *loss, float *logprob,
@@ -1084,31 +1106,22 @@ hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_pol
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
         const int64_t packs = x.vocab / Pack<T>::N;
-        if (packs <= 512)
-            launch_policy<T, 128, 4>(st, x, p, po, out, out_stride);
-        else if (packs <= 1024)
-            launch_policy<T, 256, 4>(st, x, p, po, out, out_stride);
-        else if (packs <= 4096)
-            launch_policy<T, 512, 8>(st, x, p, po, out, out_stride);
-        else if (packs <= 8192)
-            launch_policy<T, 512, 16>(st, x, p, po, out, out_stride);
-        else if (packs <= 16384)
-            launch_policy<T, 1024, 16>(st, x, p, po, out, out_stride);
-        else
-            launch_policy<T, 1024, sizeof(T) == 4 ? 16 : 8, true>(st, x, p, po, out, out_stride);
+        if (packs <= 512) return launch_policy<T, 128, 4>(st, x, p, po, out, out_stride);
+        if (packs <= 1024) return launch_policy<T, 256, 4>(st, x, p, po, out, out_stride);
+        if (packs <= 4096) return launch_policy<T, 512, 8>(st, x, p, po, out, out_stride);
+        if (packs <= 8192) return launch_policy<T, 512, 16>(st, x, p, po, out, out_stride);
+        if (packs <= 16384) return launch_policy<T, 1024, 16>(st, x, p, po, out, out_stride);
+        return launch_policy<T, 1024, sizeof(T) == 4 ? 16 : 8, true>(st, x, p, po, out, out_stride);
     });
 }
 
 hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float *loss, float *chosen,
                                   float *rejected, float *grad) {
-    const dim3 grid((unsigned)(p.pairs ? p.pairs : 1));
+    const int64_t blocks = p.pairs ? p.pairs : 1;
     const PairOut o{loss, chosen, rejected, grad};
     // 2 x 4 tokens a thread on average; a large workgroup only for long sequences
-    if (p.tokens / grid.x > 2048)
-        k_preference_loss<1024><<<grid, 1024, 0, st>>>(p, o);
-    else
-        k_preference_loss<256><<<grid, 256, 0, st>>>(p, o);
-    return hipGetLastError();
+    return p.tokens / blocks > 2048 ? launch(k_preference_loss<1024>, blocks, 1024, st, p, o)
+                                    : launch(k_preference_loss<256>, blocks, 256, st, p, o);
 }
 
 // Whether the rows can go through the DMA kernels: 16-byte chunks of rows
@@ -1149,17 +1162,17 @@ static bool head_picks(const dlr_head &h) {
            h.rows * h.hidden_stride < (INT64_C(1) << 31);  // 32-bit places of any row
 }
 
-// Classes [first, end); tile0: the statistics' first tile.  Returns the next.
+// Classes [first, end), their statistics from `tiles` on, which moves behind them.
 template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
-static int64_t launch_head_dma(hipStream_t st, dlr_head h, int64_t first, int64_t end, const HeadPick &pick,
-                               const HeadSpace &w, int64_t tile0) {
+static hipError_t launch_head_dma(hipStream_t st, dlr_head h, int64_t first, int64_t end, const HeadPick &pick,
+                                  const HeadSpace &w, int64_t &tiles) {
     constexpr int TV = WV * MV * 16, TT = WT * MT * 16;
     static_assert(TV >= kSmallestTile, "the workspace counts on it");
     const int64_t vtiles = (end - first + TV - 1) / TV, ttiles = (h.rows + TT - 1) / TT;
     h.vocab = end;
-    k_head_dma<T, WV, WT, MV, MT, S, OCC><<<dim3((unsigned)(vtiles * ttiles)), WV * WT * 64, 0, st>>>(
-        h, first, pick, w.part + tile0 * h.rows, w.zy);
-    return tile0 + vtiles;
+    float2 *part = w.part + tiles * h.rows;
+    tiles += vtiles;
+    return launch(k_head_dma<T, WV, WT, MV, MT, S, OCC>, vtiles * ttiles, WV * WT * 64, st, h, first, pick, part, w.zy);
 }
 
 // The tiles of more than 16 rows.  What a tile costs: microseconds per stage
@@ -1219,51 +1232,47 @@ static HeadPlan head_plan(const dlr_head &h) {
 }
 
 template <typename T>
-static int64_t launch_head_tiles(hipStream_t st, const dlr_head &h, const HeadPick &pick, const HeadSpace &w) {
+static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const HeadPick &pick, const HeadSpace &w,
+                                    int64_t &tiles) {
     if (!head_by_dma(h)) {
-        const int64_t vtiles = (h.vocab + kTileV - 1) / kTileV;
-        k_head_tile<T><<<dim3((unsigned)(vtiles * ((h.rows + kTileT - 1) / kTileT))), 256, 0, st>>>(h, w.part, w.zy);
-        return vtiles;
+        tiles = (h.vocab + kTileV - 1) / kTileV;
+        return launch(k_head_tile<T>, tiles * ((h.rows + kTileT - 1) / kTileT), 256, st, h, w.part, w.zy);
     }
     // Up to 16 rows the head's bytes are all there is: 256 classes a workgroup
     // once that is most of two workgroups a CU, else 64 with a deeper queue (1
     // row x 4096: 131,072 classes 180 us against 190, 65,536 classes 118
     // against 105).
     if (h.rows <= 16)
-        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, 0, h.vocab, pick, w, 0)
-                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, 0, h.vocab, pick, w, 0);
-    auto launch = [&](int tile, int64_t first, int64_t end, int64_t tile0) {
+        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, 0, h.vocab, pick, w, tiles)
+                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, 0, h.vocab, pick, w, tiles);
+    auto by = [&](int tile, int64_t first, int64_t end) {
         switch (tile) {
-            case 0: return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, first, end, pick, w, tile0);
-            case 1: return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, first, end, pick, w, tile0);
-            case 2: return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, first, end, pick, w, tile0);
-            default: return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, first, end, pick, w, tile0);
+            case 0: return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, first, end, pick, w, tiles);
+            case 1: return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, first, end, pick, w, tiles);
+            case 2: return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, first, end, pick, w, tiles);
+            default: return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, first, end, pick, w, tiles);
         }
     };
     const HeadPlan plan = head_plan(h);
-    int64_t tiles = launch(plan.first, 0, plan.classes, 0);
-    if (plan.classes < h.vocab) tiles = launch(plan.rest, plan.classes, h.vocab, tiles);
-    return tiles;
+    const hipError_t e = by(plan.first, 0, plan.classes);
+    return e != hipSuccess || plan.classes == h.vocab ? e : by(plan.rest, plan.classes, h.vocab);
 }
 
 hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
     const HeadSpace w = head_space(workspace, h.rows);
     const bool picks = head_by_dma(h) && head_picks(h);
     const HeadPick pick{picks ? w.row : nullptr, w.count};
-    hipError_t e;
-    if (picks) {
-        k_head_pick<<<1, 1024, 0, st>>>(h.target, h.target_bits, h.rows, w.row, w.count, logprob, lse);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
-    const int64_t tiles = h.dtype == DLR_DTYPE_BF16 ? launch_head_tiles<__bf16>(st, h, pick, w)
-                                                    : launch_head_tiles<_Float16>(st, h, pick, w);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    if (h.rows < 16)
-        k_head_join<1><<<dim3((unsigned)h.rows), 256, 0, st>>>(h, pick, tiles, w.part, w.zy, logprob, lse);
-    else
-        k_head_join<16><<<dim3((unsigned)((h.rows + 15) / 16)), 256, 0, st>>>(h, pick, tiles, w.part, w.zy, logprob,
-                                                                               lse);
-    return hipGetLastError();
+    hipError_t e = hipSuccess;
+    if (picks)
+        e = launch(k_head_pick, 1, 1024, st, h.target, h.target_bits, h.rows, w.row, w.count, logprob, lse);
+    int64_t tiles = 0;
+    if (e == hipSuccess)
+        e = h.dtype == DLR_DTYPE_BF16 ? launch_head_tiles<__bf16>(st, h, pick, w, tiles)
+                                      : launch_head_tiles<_Float16>(st, h, pick, w, tiles);
+    if (e != hipSuccess) return e;
+    return h.rows < 16 ? launch(k_head_join<1>, h.rows, 256, st, h, pick, tiles, w.part, w.zy, logprob, lse)
+                       : launch(k_head_join<16>, (h.rows + 15) / 16, 256, st, h, pick, tiles, w.part, w.zy, logprob,
+                                lse);
 }
 
 }  // namespace dlr

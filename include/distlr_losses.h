@@ -66,10 +66,10 @@ typedef struct dlr_logits {
     const void *target;     /* rows class indices; < 0: the row takes no part */
     int64_t rows;
     int64_t vocab;          /* classes, 1 .. 2^30                             */
-    int64_t row_stride;     /* elements, >= vocab (or 0: one row for all)     */
+    int64_t row_stride;     /* elements, >= vocab (0: one row for all)        */
     int32_t dtype;          /* DLR_DTYPE_*                                    */
     int32_t target_bits;    /* 32 or 64                                       */
-    double temperature;     /* > 0, finite                                    */
+    double temperature;     /* 1e-6 .. 1e6                                    */
 } dlr_logits;
 
 /* lse[t] = log sum_j exp(z_tj / temperature), logprob[t] = z_ty / temperature

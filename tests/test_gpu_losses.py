@@ -677,3 +677,49 @@ def test_head_long_calls_leave_out_the_rows_that_take_no_part(L, out):
     e = lse_tol(vocab) + U * 3 * 12
     close(lse, want_lse, torch.where(keep, e + U * want_lse.abs(), 0.0))
     close(lp, want_lp, torch.where(keep, e + U * want_lp.abs(), 0.0))
+
+
+def test_captured_with_picked_rows(L):
+    """A captured long call, its rows picked on the device: the mask changes
+    between replays."""
+    rows, vocab, dim = 640, 50001, 2048
+    x = torch.randn(rows, dim, generator=gen(1)).bfloat16().cuda()
+    w = (torch.randn(vocab, dim, generator=gen(2)) / 18).bfloat16().cuda()
+    y = make_target(rows, vocab).cuda()
+    L.head_logprob(x, w, y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = L.head_logprob(x, w, y)
+    for seed in range(4):
+        new = make_target(rows, vocab, seed + 5)
+        new[torch.rand(rows, generator=gen(seed)) < 0.3 * seed] = -1
+        y.copy_(new)
+        want = [t.clone() for t in L.head_logprob(x, w, y)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
+
+
+def test_class_of_probability_zero(L):
+    # the given class is masked out for the policy: the KL estimate is inf, not NaN
+    z, _ = make_logits(3, 50, torch.float32)
+    y = torch.tensor([4, 5, 6]).cuda()
+    z[1, 5] = float("-inf")
+    v = torch.full((3,), -2.0).cuda()
+    out = L.policy_loss(z, y, v, torch.ones(3).cuda(), ref_logprob=v, kl_coef=0.1)
+    assert out.kl[1] == float("inf") and out.loss[1] == float("inf") and out.logprob[1] == float("-inf")
+    assert torch.isfinite(out.grad[[0, 2]]).all() and torch.isfinite(out.kl[[0, 2]]).all()
+    quiet = L.policy_loss(z, y, v, torch.ones(3).cuda(), ref_logprob=v)  # reported, but no term of the loss
+    assert quiet.kl[1] == float("inf") and quiet.loss[1] == 0 and torch.isfinite(quiet.grad).all()
+
+
+def test_the_current_device_and_the_last_error_stay(L, dlr):
+    z, y = torch.zeros(3, 5).cuda(), torch.zeros(3, dtype=torch.int64).cuda()
+    x = L._logits(z, y, 1.0)[2]
+    import ctypes
+    assert L.lib.dlr_token_logprob(99, None, ctypes.byref(x), z.data_ptr(), z.data_ptr()) == -4
+    assert torch.cuda.current_device() == 0
+    torch.cuda.synchronize()  # the failed call's error is not reported again
+    lp, _ = L.token_logprob(z, y)
+    assert abs(float(lp[0]) + math.log(5)) < 1e-6

@@ -175,6 +175,18 @@ def test_head_workspace():
         assert rc == dlr.E_ARG and "workspace" in msg
 
 
+def test_a_device_that_is_not_there():
+    x, p = logits(), L._Policy(D, None, D, None, 0.2, 0.2, 0.0)
+    q = L._Preference(A, None, None, B, None, 2, 10, 0.1, 0.0, 0.0, 0, 0)
+    h = L._Head(A, A, B, 4, 100, 64, 64, 64, L.DTYPE_BF16, 64, 1.0)
+    for rc in (L.lib.dlr_token_logprob(99, None, C.byref(x), D, E),
+               L.lib.dlr_token_logprob_grad(99, None, C.byref(x), D, D, E, 8),
+               L.lib.dlr_policy_loss(99, None, C.byref(x), C.byref(p), E, E, E, E, None, 0),
+               L.lib.dlr_preference_loss(99, None, C.byref(q), D, D, D, E),
+               L.lib.dlr_head_logprob(99, None, C.byref(h), D, 1 << 20, E, E)):
+        assert code(rc)[0] == -4  # DLR_E_HIP
+
+
 def test_no_rows_is_a_valid_call():
     x, p = logits(rows=0, data=None, target=None), L._Policy(None, None, None, None, 0.2, 0.2, 0.0)
     assert L.lib.dlr_token_logprob(0, None, C.byref(x), None, None) == 0
