@@ -33,10 +33,12 @@
  *   - Errors: DLR_E_ARG for arguments that do not fit (message through
  *     dlr_losses_last_error()), nothing is enqueued then; DLR_E_HIP if the launch
  *     fails.  rows = 0 is a valid call that does nothing.
- *   - A library of its own, because it shares its caller's HIP runtime: its
- *     streams and tensors are the caller's.  It is linked to the name
- *     "libamdhip64.so", under which torch loads its runtime, so in a process
- *     with torch it is torch's, whatever libdistlr_amd.so is bound to.
+ *   - A library of its own: it needs neither the engine nor RCCL, and it
+ *     shares its caller's HIP runtime, whose streams and tensors it takes.  It
+ *     is linked to the name "libamdhip64.so", under which torch loads its
+ *     runtime.  A process that also runs the engine imports torch before
+ *     distlr_amd (libdistlr_amd.so then takes torch's runtime too): of two HIP
+ *     runtimes in a process only one sees the GPU.
  */
 #ifndef DISTLR_LOSSES_H_
 #define DISTLR_LOSSES_H_

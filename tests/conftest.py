@@ -12,6 +12,11 @@ import sys
 
 import pytest
 
+try:  # before any test imports distlr_amd, as bench.py and smoke() do: the process then has one HIP runtime
+    import torch  # noqa: F401  (a second one in a process does not see the GPU)
+except ImportError:
+    pass
+
 ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 GOLDEN = os.path.join(ROOT, "tests", "golden")
 sys.path.insert(0, os.path.join(ROOT, "dist-lr_amd"))

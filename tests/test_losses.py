@@ -36,6 +36,12 @@ def test_header_library_and_binding_agree():
         assert b"amdgcn-amd-amdhsa--gfx950" in f.read()
 
 
+@pytest.mark.parametrize("language", ["c", "c++"])
+def test_header_stands_alone(language):
+    subprocess.run(["g++", "-fsyntax-only", "-Wall", "-Werror", "-x", language, "-I", os.path.join(ROOT, "include"), "-"],
+                   input=b'#include "distlr_losses.h"\n', check=True)
+
+
 @pytest.mark.parametrize("order", ["torch, distlr_amd.losses", "distlr_amd, torch, distlr_amd.losses",
                                    "distlr_amd.losses"])
 def test_the_library_takes_torchs_runtime_in_any_order_of_imports(order):
