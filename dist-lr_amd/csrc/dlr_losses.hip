@@ -778,43 +778,48 @@ __global__ __launch_bounds__(1024) void k_head_pick(const void *target, int targ
 #define SCHED_DMA(n) __builtin_amdgcn_sched_group_barrier(32, n, 0)
 #define SCHED_LDS(n) __builtin_amdgcn_sched_group_barrier(256, n, 0)
 
-template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
-__global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int64_t v_first, HeadPick pick, float2 *part,
-                                                               float *zy) {
+// Measured (bf16): 256 x 256 tiles, 8 waves of 128 x 64, 4096 x 4096 x 65536
+// 1.59 ms, 1,380 TFLOP/s, softmax included, where the library's product alone
+// takes 1.54; the matrix cores are busy 60% of the time at 2.0 GHz and LDS
+// reads about as long.  4 waves of 128 x 128 read a third less from LDS, but
+// the compiler then moves accumulators between register files (994 TFLOP/s);
+// 32 x 32 products meet LDS banks twice in this layout (1,109); a workgroup
+// that goes on to its next tile and fetches it under this one's end spills
+// (1,105).  The groups' order below was the best of eleven (1,310 .. 1,380).
+// Few rows: bound by the head's bytes, 1 x 4096 x 131072 178 us (6.0 TB/s).
+template <typename T, int WV, int WT, int MV, int MT, int S>
+__global__ __launch_bounds__(WV *WT * 64) void k_head_dma(dlr_head h, int64_t v_first, HeadPick pick, float2 *part,
+                                                          float *zy) {
     constexpr int NW = WV * WT, TV = WV * MV * 16, TT = WT * MT * 16, kRow = 128;
     constexpr int kLoads = (TV + TT) / 8, L = (kLoads + NW - 1) / NW;  // DMA loads of 8 rows: all, a wave's
-    static_assert(TV % 8 == 0 && TT % 8 == 0 && S >= 2 && L * (S - 2) < 64, "whole loads, a wait that can be written");
+    static_assert(TV % 8 == 0 && TT % 8 == 0 && S >= 2 && L * (S - 1) < 64, "whole loads, a wait that can be written");
     __shared__ __attribute__((aligned(256))) char sm[S][(TV + TT) * kRow];
+    RowStat *stat = reinterpret_cast<RowStat *>(sm[0]);  // [WV][TT], behind the products
+    static_assert(sizeof(RowStat) * WV * TT <= sizeof sm, "they fit");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wv = wave / WT, wt = wave % WT;
     const int64_t used = pick.row ? *pick.count : h.rows;
-    const int64_t vtiles = (h.vocab - v_first + TV - 1) / TV, ttiles = (used + TT - 1) / TT;
-    // XCD x takes a contiguous piece of the tile order, in which up to 8
-    // token tiles of one class tile follow each other: an XCD's 32 running
-    // workgroups share 8 token and 4 class tiles in its L2.
-    int64_t tile = blockIdx.x;
-    {
-        const int64_t n = vtiles * ttiles, q = n / 8, rem = n % 8, x = tile % 8;
-        if (tile >= n) return;  // the launch counts all rows
-        tile = x * q + (x < rem ? x : rem) + tile / 8;
-    }
-    const int64_t group = vtiles * 8;  // tiles of 8 token tiles' group
-    const int64_t g = tile / group;
+    const int64_t vtiles = (h.vocab - v_first + TV - 1) / TV, ttiles = (used + TT - 1) / TT, tiles = vtiles * ttiles;
+    if (blockIdx.x >= tiles) return;  // the launch counts all rows
+    // XCD x takes a contiguous piece of the tile order, in which up to 8 token
+    // tiles of one class tile follow each other: an XCD's 32 running workgroups
+    // share 8 token and 4 class tiles in its L2.
+    const int64_t q8 = tiles / 8, rem = tiles % 8, x8 = blockIdx.x % 8;
+    const int64_t tile = x8 * q8 + (x8 < rem ? x8 : rem) + blockIdx.x / 8;
+    const int64_t group = vtiles * 8, g = tile / group;  // tiles of 8 token tiles' group
     const int in_g = ttiles - g * 8 < 8 ? (int)(ttiles - g * 8) : 8;
     const int64_t rest = tile - g * group;
-    const int64_t vt = rest / in_g, tt = g * 8 + rest % in_g;
-    const int64_t v0 = v_first + vt * TV, t0 = tt * TT;
+    // the same in every lane, which the divisions do not show: scalar registers
+    const int64_t vt = __builtin_amdgcn_readfirstlane((int)(rest / in_g)), v0 = v_first + vt * TV;
+    const int64_t t0 = (int64_t)__builtin_amdgcn_readfirstlane((int)(g * 8 + rest % in_g)) * TT;
     const int dim = (int)h.dim, full = dim / 64, steps = (dim + 63) / 64;
-
-    // This lane's places in the wave's DMA loads, from the tile's first row.
-    // Rows outside repeat the last one; a wave without an L-th load repeats
-    // the last load (every wave then has L of them in flight per stage).
-    const char *base_v = static_cast<const char *>(h.head) + v0 * h.head_stride * 2;
     const bool picked = pick.row && used < h.rows;  // all of them: in their places, without a trip to the list
-    const int64_t t_base = picked ? 0 : t0;
-    const char *base_t = static_cast<const char *>(h.hidden) + t_base * h.hidden_stride * 2;
     auto token = [&](int64_t t) { return picked ? (int64_t)pick.row[t] : t; };
-    uint32_t off[L];
+
+    // This lane's places in the wave's DMA loads.  Rows outside repeat the last
+    // one; a wave without an L-th load repeats the last load (every wave then
+    // has L of them in flight per stage).
+    const char *src[L];  // of the stage to be filled next
     const int chunk = (lane & 7) ^ (lane >> 3);
     auto load_no = [&](int q) {
         const int n = wave * L + q;
@@ -825,22 +830,26 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int64
         const int n = load_no(q);
         const bool x = n >= TV / 8;
         const int r = (x ? n - TV / 8 : n) * 8 + (lane >> 3);
-        const int64_t last = x ? used - 1 - t0 : h.vocab - 1 - v0;
-        const int64_t at = r < last ? r : last;
-        off[q] = (uint32_t)((x ? (token(t0 + at) - t_base) * h.hidden_stride : at * h.head_stride) * 2 + chunk * 16);
+        const int64_t first = x ? t0 : v0, last = (x ? used : h.vocab) - 1;
+        int64_t at = first + r < last ? first + r : last;
+        if (x) at = token(at);
+        src[q] = static_cast<const char *>(x ? h.hidden : h.head) + at * (x ? h.hidden_stride : h.head_stride) * 2 +
+                 chunk * 16;
     }
-    auto fill = [&](int step, int buf) {
-        const char *sv = base_v + (int64_t)step * 128, *st = base_t + (int64_t)step * 128;
+    auto fill = [&](int buf) {
 #pragma unroll
-        for (int q = 0; q < L; ++q) lds_dma16((load_no(q) >= TV / 8 ? st : sv) + off[q], sm[buf] + load_no(q) * 1024);
+        for (int q = 0; q < L; ++q) {
+            lds_dma16(src[q], sm[buf] + load_no(q) * 1024);
+            src[q] += 128;
+        }
     };
     auto fill_last = [&](int step, int buf) {  // a stage that may be short (dim is a multiple of 8): zeros behind it
         const bool in = step * 64 + chunk * 8 < dim;
-        const char *sv = base_v + (int64_t)step * 128, *st = base_t + (int64_t)step * 128;
 #pragma unroll
-        for (int q = 0; q < L; ++q)
-            lds_dma16(in ? (load_no(q) >= TV / 8 ? st : sv) + off[q] : (const char *)&kZero16,
-                      sm[buf] + load_no(q) * 1024);
+        for (int q = 0; q < L; ++q) {
+            lds_dma16(in ? src[q] : (const char *)&kZero16, sm[buf] + load_no(q) * 1024);
+            src[q] += 128;
+        }
     };
     struct Frag {
         u32x4 a[MV], b[MT];
@@ -874,10 +883,18 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int64
         asm volatile("" ::: "memory");                                                             \
     } while (0)
     Frag f0, f1;
+    if (full >= S) {
 #pragma unroll
-    for (int p = 0; p < S; ++p)
-        if (p < steps) fill_last(p, p);
-    MEET(0);
+        for (int p = 0; p < S; ++p) fill(p);
+    } else {
+#pragma unroll
+        for (int p = 0; p < S; ++p)
+            if (p < steps) fill_last(p, p);
+    }
+    if (steps >= S)
+        MEET(L *(S - 1));  // the first stage has landed
+    else
+        MEET(0);
     read(f0, 0, 0);
     int step = 0, buf = 0;
     for (; step + S < full; ++step) {
@@ -890,7 +907,7 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int64
             SCHED_MFMA(2);
         }
         MEET(L *(S - 2));
-        fill(step + S, buf);
+        fill(buf);
         read(f0, next, 0);
         multiply(f1);
 #pragma unroll
@@ -919,21 +936,20 @@ __global__ __launch_bounds__(WV *WT * 64, OCC) void k_head_dma(dlr_head h, int64
     __syncthreads();  // sm is free
     // per token (a lane column) over this wave's classes, then over the waves
     const ExpScale k = exp_scale(h.temperature);
-    RowStat *stat = reinterpret_cast<RowStat *>(sm[0]);  // [WV][TT]
-    const bool ragged = v0 + TV > h.vocab;
+    const int classes = h.vocab - v0 < TV ? (int)(h.vocab - v0) : TV, base = wv * MV * 16 + (lane >> 4) * 4;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
         const int64_t t = t0 + wt * MT * 16 + j * 16 + (lane & 15);
         const int64_t row = t < used ? token(t) : -1;
-        const int64_t y = row >= 0 ? load_target(h.target, h.target_bits, row) : -1;
-        const int64_t base = v0 + wv * MV * 16 + (lane >> 4) * 4;
+        const int64_t y = (row >= 0 ? load_target(h.target, h.target_bits, row) : -1) - v0;
+        const int target = y >= 0 && y < TV ? (int)y : -1;  // in the tile
         float m = NEG_INF;
 #pragma unroll
         for (int i = 0; i < MV; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (ragged && base + i * 16 + e >= h.vocab) acc[i][j][e] = NEG_INF;
-                if (base + i * 16 + e == y) zy[row] = acc[i][j][e];
+                if (classes < TV && base + i * 16 + e >= classes) acc[i][j][e] = NEG_INF;
+                if (base + i * 16 + e == target) zy[row] = acc[i][j][e];
                 m = fmaxf(m, acc[i][j][e]);
             }
         m = fmaxf(m, __shfl_xor(m, 16));
@@ -1124,14 +1140,14 @@ hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float
                                     : launch(k_preference_loss<256>, blocks, 256, st, p, o);
 }
 
-// Whether the rows can go through the DMA kernels: 16-byte chunks of rows
-// that start at 16 bytes, 32-bit places within a tile.
+// Whether the rows can go through the DMA kernels: 16-byte chunks of rows that
+// start at 16 bytes.
 static bool head_by_dma(const dlr_head &h) {
     return (reinterpret_cast<uintptr_t>(h.head) | reinterpret_cast<uintptr_t>(h.hidden)) % 16 == 0 &&
-           h.head_stride % 8 == 0 && h.hidden_stride % 8 == 0 && h.dim % 8 == 0 && h.head_stride <= (1 << 21) &&
-           h.hidden_stride <= (1 << 21);
+           h.head_stride % 8 == 0 && h.hidden_stride % 8 == 0 && h.dim % 8 == 0;
 }
 
+constexpr int64_t kCus = 256;
 constexpr int kSmallestTile = 64;  // classes: the most tiles, for the workspace
 
 // The workspace: the targets' logits, the picked rows and their count, the
@@ -1158,12 +1174,11 @@ static HeadSpace head_space(void *workspace, int64_t rows) {
 // Whether the rows that take part are picked first, so that the others cost
 // nothing: 4 us for what may be half of a long call, from about 100 us on.
 static bool head_picks(const dlr_head &h) {
-    return (double)h.rows * (double)h.vocab * (double)h.dim >= 6.4e10 && h.rows > 64 &&
-           h.rows * h.hidden_stride < (INT64_C(1) << 31);  // 32-bit places of any row
+    return (double)h.rows * (double)h.vocab * (double)h.dim >= 6.4e10 && h.rows > 64;
 }
 
 // Classes [first, end), their statistics from `tiles` on, which moves behind them.
-template <typename T, int WV, int WT, int MV, int MT, int S, int OCC>
+template <typename T, int WV, int WT, int MV, int MT, int S>
 static hipError_t launch_head_dma(hipStream_t st, dlr_head h, int64_t first, int64_t end, const HeadPick &pick,
                                   const HeadSpace &w, int64_t &tiles) {
     constexpr int TV = WV * MV * 16, TT = WT * MT * 16;
@@ -1172,7 +1187,7 @@ static hipError_t launch_head_dma(hipStream_t st, dlr_head h, int64_t first, int
     h.vocab = end;
     float2 *part = w.part + tiles * h.rows;
     tiles += vtiles;
-    return launch(k_head_dma<T, WV, WT, MV, MT, S, OCC>, vtiles * ttiles, WV * WT * 64, st, h, first, pick, part, w.zy);
+    return launch(k_head_dma<T, WV, WT, MV, MT, S>, vtiles * ttiles, WV * WT * 64, st, h, first, pick, part, w.zy);
 }
 
 // The tiles of more than 16 rows.  What a tile costs: microseconds per stage
@@ -1183,7 +1198,6 @@ struct HeadTile {
     double alone, two;  // two 0: one workgroup a CU
 };
 constexpr HeadTile kHeadTiles[] = {{256, 256, 1.56, 0}, {256, 128, 0.9, 0}, {128, 64, 0.42, 0.67}, {64, 64, 0.3, 0.55}};
-constexpr int64_t kCus = 256;
 constexpr double kEnds = 3, kLaunch = 3;
 
 static double head_cost(const HeadTile &t, int64_t rows, int64_t classes, int64_t stages) {
@@ -1243,14 +1257,14 @@ static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const Hea
     // row x 4096: 131,072 classes 180 us against 190, 65,536 classes 118
     // against 105).
     if (h.rows <= 16)
-        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2, 2>(st, h, 0, h.vocab, pick, w, tiles)
-                                         : launch_head_dma<T, 4, 1, 1, 1, 4, 4>(st, h, 0, h.vocab, pick, w, tiles);
+        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2>(st, h, 0, h.vocab, pick, w, tiles)
+                                         : launch_head_dma<T, 4, 1, 1, 1, 4>(st, h, 0, h.vocab, pick, w, tiles);
     auto by = [&](int tile, int64_t first, int64_t end) {
         switch (tile) {
-            case 0: return launch_head_dma<T, 2, 4, 8, 4, 2, 1>(st, h, first, end, pick, w, tiles);
-            case 1: return launch_head_dma<T, 4, 2, 4, 4, 3, 1>(st, h, first, end, pick, w, tiles);
-            case 2: return launch_head_dma<T, 4, 1, 2, 4, 3, 2>(st, h, first, end, pick, w, tiles);
-            default: return launch_head_dma<T, 4, 1, 1, 4, 4, 2>(st, h, first, end, pick, w, tiles);
+            case 0: return launch_head_dma<T, 2, 4, 8, 4, 2>(st, h, first, end, pick, w, tiles);
+            case 1: return launch_head_dma<T, 4, 2, 4, 4, 3>(st, h, first, end, pick, w, tiles);
+            case 2: return launch_head_dma<T, 4, 1, 2, 4, 3>(st, h, first, end, pick, w, tiles);
+            default: return launch_head_dma<T, 4, 1, 1, 4, 4>(st, h, first, end, pick, w, tiles);
         }
     };
     const HeadPlan plan = head_plan(h);
