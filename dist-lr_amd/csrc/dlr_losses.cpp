@@ -203,7 +203,7 @@ int64_t dlr_head_logprob_workspace(int64_t rows, int64_t vocab, int64_t dim) {
     if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || dim < 1 || dim > kMaxDim ||
         rows * vocab > kMaxLogits)
         return refuse(DLR_E_ARG, "dlr_head_logprob_workspace", "rows, vocab or dim is out of range");
-    return dlr::head_workspace(rows, vocab);
+    return dlr::head_workspace(rows, vocab, dim);
 }
 
 int dlr_head_logprob(int device, void *stream, const dlr_head *h, void *workspace, int64_t workspace_bytes,
@@ -228,7 +228,7 @@ int dlr_head_logprob(int device, void *stream, const dlr_head *h, void *workspac
     if (const char *why = check_target(h->target, h->target_bits, h->temperature)) return refuse(DLR_E_ARG, call, why);
     if (!logprob || !lse) return refuse(DLR_E_ARG, call, "logprob or lse is NULL");
     if (!floats({logprob, lse})) return refuse(DLR_E_ARG, call, "logprob or lse is not aligned");
-    if (!workspace || workspace_bytes < dlr::head_workspace(h->rows, h->vocab))
+    if (!workspace || workspace_bytes < dlr::head_workspace(h->rows, h->vocab, h->dim))
         return refuse(DLR_E_ARG, call, "the workspace is smaller than dlr_head_logprob_workspace");
     if (!aligned(workspace, 256)) return refuse(DLR_E_ARG, call, "the workspace is not 256-byte aligned");
     DeviceScope d(device);

@@ -20,7 +20,7 @@ hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float
                                   float *rejected, float *grad);
 
 // Bytes of launch_head_logprob's workspace.
-int64_t head_workspace(int64_t rows, int64_t vocab);
+int64_t head_workspace(int64_t rows, int64_t vocab, int64_t dim);
 hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse);
 
 }  // namespace dlr

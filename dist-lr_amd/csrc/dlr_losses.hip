@@ -1116,6 +1116,12 @@ static hipError_t launch_policy(hipStream_t st, const dlr_logits &x, const dlr_p
                   static_cast<T *>(out), out_stride);
 }
 
+// The smallest workgroup whose registers hold a row: the more of them on a CU,
+// the more of a row's two passes overlap with other rows' memory (bf16, us, the
+// row held by 512 / 1,024 threads: 4,096 x 65,536 204 / 254, 8,192 x 32,000 186
+// / 189; 8,000 x 1,000 by 128 / 256: 14 / 18).  Rows longer than a CU's
+// registers hold what fits beside the second reading's own (16 packs a thread
+// spill 16-bit types there: 1,024 x 200,000 386 us, with 8 204).
 hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, float *loss, float *logprob,
                               float *kl, uint8_t *clipped, void *out, int64_t out_stride) {
     const PolicyOut po{loss, logprob, kl, clipped};
@@ -1148,7 +1154,6 @@ static bool head_by_dma(const dlr_head &h) {
 }
 
 constexpr int64_t kCus = 256;
-constexpr int kSmallestTile = 64;  // classes: the most tiles, for the workspace
 
 // The workspace: the targets' logits, the picked rows and their count, the
 // tiles' statistics.
@@ -1159,11 +1164,6 @@ struct HeadSpace {
     float2 *part;
 };
 static int64_t head_part(int64_t rows) { return (rows * 8 + 8 + 255) / 256 * 256; }  // where the statistics begin
-
-int64_t head_workspace(int64_t rows, int64_t vocab) {
-    const int64_t tiles = (vocab + kSmallestTile - 1) / kSmallestTile;
-    return head_part(rows) + rows * tiles * (int64_t)sizeof(float2);
-}
 
 static HeadSpace head_space(void *workspace, int64_t rows) {
     char *w = static_cast<char *>(workspace);
@@ -1182,7 +1182,6 @@ template <typename T, int WV, int WT, int MV, int MT, int S>
 static hipError_t launch_head_dma(hipStream_t st, dlr_head h, int64_t first, int64_t end, const HeadPick &pick,
                                   const HeadSpace &w, int64_t &tiles) {
     constexpr int TV = WV * MV * 16, TT = WT * MT * 16;
-    static_assert(TV >= kSmallestTile, "the workspace counts on it");
     const int64_t vtiles = (end - first + TV - 1) / TV, ttiles = (h.rows + TT - 1) / TT;
     h.vocab = end;
     float2 *part = w.part + tiles * h.rows;
@@ -1200,9 +1199,11 @@ struct HeadTile {
 constexpr HeadTile kHeadTiles[] = {{256, 256, 1.56, 0}, {256, 128, 0.9, 0}, {128, 64, 0.42, 0.67}, {64, 64, 0.3, 0.55}};
 constexpr double kEnds = 3, kLaunch = 3;
 
+static int64_t tiles_of(int64_t classes, int64_t tv) { return (classes + tv - 1) / tv; }
+
 static double head_cost(const HeadTile &t, int64_t rows, int64_t classes, int64_t stages) {
     if (classes <= 0) return 0;
-    const int64_t n = ((classes + t.tv - 1) / t.tv) * ((rows + t.tt - 1) / t.tt);
+    const int64_t n = tiles_of(classes, t.tv) * tiles_of(rows, t.tt);
     if (t.two == 0 || n <= kCus) return (double)((n + kCus - 1) / kCus) * (t.alone * stages + kEnds);
     return (double)((n + 2 * kCus - 1) / (2 * kCus)) * (t.two * stages + kEnds);
 }
@@ -1216,33 +1217,50 @@ struct HeadPlan {
 // The cheapest tile for all classes, or a large one for as many classes as
 // fill whole rounds of the CUs and the cheapest for the others: 333 x 1536 x
 // 50257 is 2.3 rounds of 256 x 128 tiles, paid as 3 (74 us), or one round of
-// 256 x 256 tiles and one of 256 x 128.
-static HeadPlan head_plan(const dlr_head &h) {
-    const int64_t stages = (h.dim + 63) / 64;
+// 256 x 256 tiles and one of 256 x 128 (71).  200 x 4096 x 32000: 63 us by 256
+// x 128, 95 by 256 x 256; 2048 x 4096 x 1000: 30 us by 128 x 64, 81.
+static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t dim) {
+    const int64_t stages = (dim + 63) / 64;
     auto best = [&](int64_t classes) {
         int i = 0;
         for (int j = 1; j < 4; ++j)
-            if (head_cost(kHeadTiles[j], h.rows, classes, stages) < head_cost(kHeadTiles[i], h.rows, classes, stages))
+            if (head_cost(kHeadTiles[j], rows, classes, stages) < head_cost(kHeadTiles[i], rows, classes, stages))
                 i = j;
         return i;
     };
-    const int whole = best(h.vocab);
-    HeadPlan plan{whole, whole, h.vocab};
-    double cost = head_cost(kHeadTiles[whole], h.rows, h.vocab, stages);
+    const int whole = best(vocab);
+    HeadPlan plan{whole, whole, vocab};
+    double cost = head_cost(kHeadTiles[whole], rows, vocab, stages);
     for (int i = 0; i < 2; ++i) {
         const HeadTile &t = kHeadTiles[i];
-        const int64_t ttiles = (h.rows + t.tt - 1) / t.tt, rounds = h.vocab / t.tv * ttiles / kCus;
+        const int64_t ttiles = (rows + t.tt - 1) / t.tt, rounds = vocab / t.tv * ttiles / kCus;
         const int64_t classes = rounds * kCus / ttiles * t.tv;
-        if (classes <= 0 || classes >= h.vocab) continue;
-        const int rest = best(h.vocab - classes);
-        const double c = head_cost(t, h.rows, classes, stages) + kLaunch +
-                         head_cost(kHeadTiles[rest], h.rows, h.vocab - classes, stages);
+        if (classes <= 0 || classes >= vocab) continue;
+        const int rest = best(vocab - classes);
+        const double c = head_cost(t, rows, classes, stages) + kLaunch +
+                         head_cost(kHeadTiles[rest], rows, vocab - classes, stages);
         if (c < cost) {
             plan = {i, rest, classes};
             cost = c;
         }
     }
     return plan;
+}
+
+// Up to 16 rows the head's bytes are all there is: 256 classes a workgroup once
+// that is most of two workgroups a CU, else 64 with a deeper queue (1 row x
+// 4096: 131,072 classes 180 us against 190, 65,536 classes 118 against 105).
+static int64_t few_rows_tile(int64_t vocab) { return vocab >= 2 * kCus * 192 ? 256 : 64; }
+
+int64_t head_workspace(int64_t rows, int64_t vocab, int64_t dim) {
+    int64_t tiles = tiles_of(vocab, few_rows_tile(vocab));
+    if (rows > 16) {
+        const HeadPlan plan = head_plan(rows, vocab, dim);
+        tiles = tiles_of(plan.classes, kHeadTiles[plan.first].tv) +
+                tiles_of(vocab - plan.classes, kHeadTiles[plan.rest].tv);
+    }
+    const int64_t plain = tiles_of(vocab, kTileV);  // unaligned rows
+    return head_part(rows) + rows * (tiles > plain ? tiles : plain) * (int64_t)sizeof(float2);
 }
 
 template <typename T>
@@ -1252,12 +1270,8 @@ static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const Hea
         tiles = (h.vocab + kTileV - 1) / kTileV;
         return launch(k_head_tile<T>, tiles * ((h.rows + kTileT - 1) / kTileT), 256, st, h, w.part, w.zy);
     }
-    // Up to 16 rows the head's bytes are all there is: 256 classes a workgroup
-    // once that is most of two workgroups a CU, else 64 with a deeper queue (1
-    // row x 4096: 131,072 classes 180 us against 190, 65,536 classes 118
-    // against 105).
     if (h.rows <= 16)
-        return h.vocab >= 2 * kCus * 192 ? launch_head_dma<T, 8, 1, 2, 1, 2>(st, h, 0, h.vocab, pick, w, tiles)
+        return few_rows_tile(h.vocab) == 256 ? launch_head_dma<T, 8, 1, 2, 1, 2>(st, h, 0, h.vocab, pick, w, tiles)
                                          : launch_head_dma<T, 4, 1, 1, 1, 4>(st, h, 0, h.vocab, pick, w, tiles);
     auto by = [&](int tile, int64_t first, int64_t end) {
         switch (tile) {
@@ -1267,7 +1281,7 @@ static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const Hea
             default: return launch_head_dma<T, 4, 1, 1, 4, 4>(st, h, first, end, pick, w, tiles);
         }
     };
-    const HeadPlan plan = head_plan(h);
+    const HeadPlan plan = head_plan(h.rows, h.vocab, h.dim);
     const hipError_t e = by(plan.first, 0, plan.classes);
     return e != hipSuccess || plan.classes == h.vocab ? e : by(plan.rest, plan.classes, h.vocab);
 }

@@ -159,6 +159,8 @@ def _grad_like(logits: torch.Tensor, out: Optional[torch.Tensor], gpu: int) -> t
     _matrix("out", out, gpu)
     if out.dtype != logits.dtype or out.shape != logits.shape:
         _refuse("out must have the logits' type and shape")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)  # autograd sees that a tensor it may have saved is written
     return out
 
 

@@ -25,6 +25,7 @@
  *     marks a row that takes no part: its logits are not read (NaN there does
  *     no harm), its results are 0 and its gradient's row is 0.  A target >=
  *     vocab gives NaN (nothing is read out of range).
+ *   - The arrays of a call do not overlap, except where a call says so.
  *   - -inf logits (classes masked out) have probability 0.  A row of -inf
  *     only has lse -inf and logprob NaN; NaN or +inf in a row make it NaN.
  *   - Row statistics are held in 32 bits and finished in 64; gradients are

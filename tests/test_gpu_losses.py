@@ -723,3 +723,91 @@ def test_the_current_device_and_the_last_error_stay(L, dlr):
     torch.cuda.synchronize()  # the failed call's error is not reported again
     lp, _ = L.token_logprob(z, y)
     assert abs(float(lp[0]) + math.log(5)) < 1e-6
+
+
+def test_targets_of_32_bits_and_strided_vectors(L):
+    z, _ = make_logits(11, 300, torch.bfloat16)
+    x, w = torch.randn(11, 64).bfloat16().cuda(), torch.randn(300, 64).bfloat16().cuda()
+    y = make_target(11, 300, ignore=(2,)).cuda()
+    v = torch.randn(5, 11, generator=gen(3)).cuda()
+
+    def calls(y, v):
+        lp, lse = L.token_logprob(z, y)
+        g = L.token_logprob_grad(z, y, lse, v[0])
+        p = L.policy_loss(z, y, v[1] - 6, v[2], ref_logprob=v[3] - 6, weight=v[4], kl_coef=0.1)
+        q = L.preference_loss(v[0], v[1], torch.tensor([0, 3, 5, 7, 11]).cuda(), beta=0.1, weight=v[2][:2])
+        return [lp, lse, g, *p, *q, *L.head_logprob(x, w, y)]
+
+    apart = v.t().contiguous().t()  # the same vectors, 5 elements apart
+    assert not apart[0].is_contiguous()
+    wide = torch.stack([y, y], 1)[:, 0]
+    for other in (calls(y.int(), v), calls(y, apart), calls(wide, v)):
+        for a, b in zip(calls(y, v), other):
+            assert torch.equal(a, b)
+
+
+def test_many_short_rows_and_pairs(L):
+    rows = 70003
+    z, z64 = make_logits(rows, 5, torch.float32)
+    y = make_target(rows, 5)
+    lp, _ = L.token_logprob(z, y.cuda())
+    want, _ = ref_logprob(z64, y, 1.0)
+    close(lp, want, lse_tol(5) + U * want.abs())
+    out = L.policy_loss(z, y.cuda(), lp, torch.ones(rows).cuda())
+    close(out.loss, torch.full((rows,), -1.0).double(), torch.tensor(2 * lse_tol(5) + 4 * U).double())  # ratio 1
+    P = 70001
+    l = torch.randn(2 * P, generator=gen(1))
+    got = L.preference_loss(l.cuda(), None, torch.arange(2 * P + 1).cuda(), beta=1.0)
+    u = l[:P].double() - l[P:].double()
+    want = torch.nn.functional.softplus(-u)
+    close(got.loss, want, 1.01 * U * want + 1e-12)
+    slope = torch.sigmoid(u) - 1
+    close(got.grad, torch.cat([slope, -slope]), 1.01 * U * slope.abs().repeat(2) + 1e-12)
+
+
+def test_two_calls_at_once(L):
+    """On two streams, each with its own scratch memory."""
+    args = []
+    for seed in (1, 2):
+        x = torch.randn(200, 512, generator=gen(seed)).bfloat16().cuda()
+        w = (torch.randn(20011, 512, generator=gen(seed + 5)) / 9).bfloat16().cuda()
+        args.append((x, w, make_target(200, 20011, seed).cuda()))
+    want = [[t.clone() for t in L.head_logprob(*a)] for a in args]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(L.head_logprob(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for out in got[i] for a, b in zip(out, want[i]))
+
+
+@pytest.mark.parametrize("rows,vocab,dim", [(333, 50257, 512), (600, 30001, 512), (700, 50257, 512)])
+def test_head_tiles_of_two_kinds(L, rows, vocab, dim):
+    # whole rounds of large tiles, the other classes by smaller ones; targets on both sides of the seam
+    g = gen(rows)
+    x = torch.randint(-2, 3, (rows, dim), generator=g).half()
+    w = torch.randint(-2, 3, (vocab, dim), generator=g).half()
+    y = make_target(rows, vocab, ignore=(7,))
+    y[0], y[1] = 0, vocab - 1
+    scale = 3 * math.sqrt(dim)
+    lp, lse = L.head_logprob(x.cuda(), w.cuda(), y.cuda(), temperature=scale)
+    want_lp, want_lse = ref_logprob((x.cuda().double() @ w.cuda().double().t()).cpu(), y, scale)
+    e = lse_tol(vocab) + U * 3 * 12
+    close(lse, want_lse, e + U * want_lse.abs())
+    close(lp, want_lp, e + U * want_lp.abs())
+
+
+def test_autograd_notices_a_gradient_written_over_the_logits(L):
+    z = torch.randn(4, 9, device="cuda", requires_grad=True)
+    h = z * 2.0
+    loss = (h * h).sum()  # saves h
+    y = make_target(4, 9).cuda()
+    lp, lse = L.token_logprob(h, y)
+    assert not lp.requires_grad
+    L.token_logprob_grad(h.detach(), y, lse, torch.ones(4).cuda(), out=h.detach())
+    with pytest.raises(RuntimeError):
+        loss.backward()
