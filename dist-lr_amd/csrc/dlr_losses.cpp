@@ -100,6 +100,13 @@ const char *check_grad(const dlr_logits *x, const void *grad, int64_t stride) {
     return nullptr;
 }
 
+const char *check_workspace(const void *workspace, int64_t bytes, int64_t need) {
+    if (need == 0) return nullptr;
+    if (!workspace || bytes < need) return "the workspace is smaller than its size call says";
+    if (!aligned(workspace, 256)) return "the workspace is not 256-byte aligned";
+    return nullptr;
+}
+
 bool floats(std::initializer_list<const void *> ps) {
     for (const void *p : ps)
         if (!aligned(p, 4)) return false;
@@ -117,15 +124,24 @@ const char *dlr_losses_runtime(void) {
     return dladdr(reinterpret_cast<const void *>(&hipGetDevice), &info) && info.dli_fname ? info.dli_fname : "";
 }
 
-int dlr_token_logprob(int device, void *stream, const dlr_logits *x, float *logprob, float *lse) {
+int64_t dlr_logits_workspace(int64_t rows, int64_t vocab, int dtype) {
+    if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || dtype < DLR_DTYPE_F32 || dtype > DLR_DTYPE_F16)
+        return refuse(DLR_E_ARG, "dlr_logits_workspace", "rows, vocab or dtype is out of range");
+    return dlr::logits_workspace(rows, vocab, dtype);
+}
+
+int dlr_token_logprob(int device, void *stream, const dlr_logits *x, void *workspace, int64_t workspace_bytes,
+                      float *logprob, float *lse) {
     const char *call = "dlr_token_logprob";
     if (const char *why = check_logits(x)) return refuse(DLR_E_ARG, call, why);
     if (x->rows == 0) return DLR_OK;
     if (!logprob || !lse) return refuse(DLR_E_ARG, call, "logprob or lse is NULL");
     if (!floats({logprob, lse})) return refuse(DLR_E_ARG, call, "logprob or lse is not aligned");
+    if (const char *why = check_workspace(workspace, workspace_bytes, dlr::logits_workspace(x->rows, x->vocab, x->dtype)))
+        return refuse(DLR_E_ARG, call, why);
     DeviceScope d(device);
     if (d.error() != hipSuccess) return fail_hip(call, d.error());
-    const hipError_t e = dlr::launch_token_logprob(static_cast<hipStream_t>(stream), *x, logprob, lse);
+    const hipError_t e = dlr::launch_token_logprob(static_cast<hipStream_t>(stream), *x, workspace, logprob, lse);
     return e == hipSuccess ? DLR_OK : fail_hip(call, e);
 }
 
@@ -144,8 +160,9 @@ int dlr_token_logprob_grad(int device, void *stream, const dlr_logits *x, const 
     return e == hipSuccess ? DLR_OK : fail_hip(call, e);
 }
 
-int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_policy *p, float *loss, float *logprob,
-                    float *kl, uint8_t *clipped, void *grad_logits, int64_t grad_row_stride) {
+int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_policy *p, void *workspace,
+                    int64_t workspace_bytes, float *loss, float *logprob, float *kl, uint8_t *clipped,
+                    void *grad_logits, int64_t grad_row_stride) {
     const char *call = "dlr_policy_loss";
     if (const char *why = check_logits(x)) return refuse(DLR_E_ARG, call, why);
     if (!p) return refuse(DLR_E_ARG, call, "the policy's descriptor is NULL");
@@ -162,10 +179,12 @@ int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_pol
         return refuse(DLR_E_ARG, call, "a float array is not aligned");
     if (grad_logits)
         if (const char *why = check_grad(x, grad_logits, grad_row_stride)) return refuse(DLR_E_ARG, call, why);
+    if (const char *why = check_workspace(workspace, workspace_bytes, dlr::logits_workspace(x->rows, x->vocab, x->dtype)))
+        return refuse(DLR_E_ARG, call, why);
     DeviceScope d(device);
     if (d.error() != hipSuccess) return fail_hip(call, d.error());
-    const hipError_t e = dlr::launch_policy_loss(static_cast<hipStream_t>(stream), *x, *p, loss, logprob, kl, clipped,
-                                                 grad_logits, grad_row_stride);
+    const hipError_t e = dlr::launch_policy_loss(static_cast<hipStream_t>(stream), *x, *p, workspace, loss, logprob, kl,
+                                                 clipped, grad_logits, grad_row_stride);
     return e == hipSuccess ? DLR_OK : fail_hip(call, e);
 }
 
@@ -228,9 +247,8 @@ int dlr_head_logprob(int device, void *stream, const dlr_head *h, void *workspac
     if (const char *why = check_target(h->target, h->target_bits, h->temperature)) return refuse(DLR_E_ARG, call, why);
     if (!logprob || !lse) return refuse(DLR_E_ARG, call, "logprob or lse is NULL");
     if (!floats({logprob, lse})) return refuse(DLR_E_ARG, call, "logprob or lse is not aligned");
-    if (!workspace || workspace_bytes < dlr::head_workspace(h->rows, h->vocab, h->dim))
-        return refuse(DLR_E_ARG, call, "the workspace is smaller than dlr_head_logprob_workspace");
-    if (!aligned(workspace, 256)) return refuse(DLR_E_ARG, call, "the workspace is not 256-byte aligned");
+    if (const char *why = check_workspace(workspace, workspace_bytes, dlr::head_workspace(h->rows, h->vocab, h->dim)))
+        return refuse(DLR_E_ARG, call, why);
     DeviceScope d(device);
     if (d.error() != hipSuccess) return fail_hip(call, d.error());
     const hipError_t e = dlr::launch_head_logprob(static_cast<hipStream_t>(stream), *h, workspace, logprob, lse);

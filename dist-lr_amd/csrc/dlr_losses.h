@@ -11,11 +11,13 @@
 
 namespace dlr {
 
-hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse);
+// Bytes of scratch memory of launch_token_logprob and launch_policy_loss.
+int64_t logits_workspace(int64_t rows, int64_t vocab, int32_t dtype);
+hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, void *workspace, float *logprob, float *lse);
 hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad,
                                      void *out, int64_t out_stride);
-hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, float *loss, float *logprob,
-                              float *kl, uint8_t *clipped, void *out, int64_t out_stride);
+hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, void *workspace, float *loss,
+                              float *logprob, float *kl, uint8_t *clipped, void *out, int64_t out_stride);
 hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float *loss, float *chosen,
                                   float *rejected, float *grad);
 

@@ -272,6 +272,69 @@ __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t s
     }
 }
 
+// ---- few long rows: a row's chunks by several workgroups
+//
+// A CU alone reads a long row slowly.  Up to 128 rows of 8,192 packs and more
+// go by chunks: their statistics to scratch memory (and the target's logit,
+// which the gradient may then overwrite), a second launch joins them.  1 x
+// 131,072 bf16: 5.9 us, 10.9 by one workgroup; the policy loss 8.6, 18.8.
+struct RowPart {
+    double s;
+    float m;
+    float pad;
+};
+struct RowParts {
+    RowPart *part;  // rows x chunks
+    float *zy;      // rows
+    int chunks, span;
+};
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_row_part(const T *logits, int64_t stride, int vocab, const void *target,
+                                                 int target_bits, const float *weight, ExpScale k, RowParts w) {
+    __shared__ BlockLds<NT> lds;
+    const int64_t t = blockIdx.x / w.chunks;
+    const int begin = (int)(blockIdx.x % w.chunks) * w.span, here = vocab - begin < w.span ? vocab - begin : w.span;
+    const int64_t y = load_target(target, target_bits, t);
+    if (y < 0 || (weight && weight[t] == 0.f)) return;
+    const T *row = logits + t * stride;
+    const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row + begin, here, k, false), k, lds);
+    if (threadIdx.x == 0) {
+        w.part[blockIdx.x] = {a.s, a.m, 0.f};
+        if (y >= begin && y < begin + here) w.zy[t] = (float)row[y];
+    }
+}
+
+// A row's chunks (at most 64) joined by one wave, in every lane.
+__device__ inline BlockStat join_parts(const RowParts &w, int64_t t, ExpScale k) {
+    const int lane = threadIdx.x & 63;
+    RowPart q{0.0, NEG_INF, 0.f};
+    if (lane < w.chunks) q = w.part[t * w.chunks + lane];
+    float m = q.m;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    double s = q.s * (double)exp2_scaled(q.m - (m == NEG_INF ? 0.f : m), k);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    return {m, s};
+}
+
+__global__ __launch_bounds__(64) void k_token_finish(const void *target, int target_bits, int vocab, ExpScale k,
+                                                     double tau, RowParts w, float *logprob, float *lse) {
+    const int64_t t = blockIdx.x;
+    const int64_t y = load_target(target, target_bits, t);
+    if (y < 0) {
+        if (threadIdx.x == 0) logprob[t] = lse[t] = 0.f;
+        return;
+    }
+    const BlockStat a = join_parts(w, t, k);
+    if (threadIdx.x == 0) {
+        const double ln = log(a.s);
+        lse[t] = (float)(a.m / tau + ln);
+        logprob[t] = (float)target_logprob(y < vocab ? w.zy[t] : __builtin_nanf(""), a.m, ln, tau);
+    }
+}
+
 // Writes `out`'s row of zeros.
 template <typename T, int NT>
 __device__ inline void zero_row(T *out, int vocab) {
@@ -328,28 +391,30 @@ template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int64_t stride, int vocab,
                                                            const void *target, int target_bits, double tau, bool once,
                                                            const float *lse, const float *grad, T *out,
-                                                           int64_t out_stride) {
-    const int64_t t = blockIdx.x;
+                                                           int64_t out_stride, int chunks, int span) {
+    const int64_t t = blockIdx.x / chunks;
+    const int begin = (int)(blockIdx.x % chunks) * span, here = vocab - begin < span ? vocab - begin : span;
     const int64_t y = load_target(target, target_bits, t);
-    T *o = out + t * out_stride;
+    T *o = out + t * out_stride + begin;
     const float g = y < 0 ? 0.f : grad[t];
     if (g == 0.f) {  // ignored, or nothing flows back: the row is not read
-        zero_row<T, NT>(o, vocab);
+        zero_row<T, NT>(o, here);
         return;
     }
+    const T *row = logits + t * stride;
     const float c = y < vocab ? (float)(g / tau) : __builtin_nanf("");
     const float l = lse[t];
     if (fabsf(l) > kLseExact) {
         __shared__ BlockLds<NT> lds;
         const ExpScale k = exp_scale(tau);
-        const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(logits + t * stride, vocab, k, false), k, lds);
+        const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k, false), k, lds);
         const float neg = (float)(-c / a.s), m = a.m;
-        residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
+        residual_row<T, NT, 4>(row + begin, o, here, y - begin, c,
                                [=](float z) { return neg * exp2_hw((z - m) * k.hi); }, once);
         return;
     }
     const float it = (float)(1.0 / tau);
-    residual_row<T, NT, 4>(logits + t * stride, o, vocab, y, c,
+    residual_row<T, NT, 4>(row + begin, o, here, y - begin, c,
                            [=](float z) { return -c * exp2_hw(__builtin_fmaf(z, it, -l) * 1.44269504f); }, once);
 }
 
@@ -361,8 +426,9 @@ struct PolicyOut {
 };
 
 // One row's loss from its log-probability, in 64 bits.  Returns d loss /
-// d logprob times the weight.
-__device__ inline double policy_token(double lp, const dlr_policy &p, int64_t t, double w, const PolicyOut &o) {
+// d logprob times the weight; `write`: this caller writes the row's results.
+__device__ inline double policy_token(double lp, const dlr_policy &p, int64_t t, double w, const PolicyOut &o,
+                                      bool write) {
     const double adv = p.advantage[t];
     const double ratio = exp(lp - (double)p.old_logprob[t]);
     const double lo = 1.0 - p.clip_low, hi = 1.0 + p.clip_high;
@@ -382,11 +448,49 @@ __device__ inline double policy_token(double lp, const dlr_policy &p, int64_t t,
         }
     }
     if (ratio != ratio) loss = slope = ratio;  // NaN log-probabilities stay visible
-    o.loss[t] = (float)loss;
-    o.logprob[t] = (float)lp;
-    o.kl[t] = (float)kl;
-    o.clipped[t] = held;
+    if (write) {
+        o.loss[t] = (float)loss;
+        o.logprob[t] = (float)lp;
+        o.kl[t] = (float)kl;
+        o.clipped[t] = held;
+    }
     return slope * w;
+}
+
+__device__ inline void policy_nothing(int64_t t, const PolicyOut &o) {
+    o.loss[t] = o.logprob[t] = o.kl[t] = 0.f;
+    o.clipped[t] = 0;
+}
+
+// The second launch over a row's chunks: each joins the statistics and writes
+// its part of the gradient, the first also the row's results.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_policy_finish(const T *logits, int64_t stride, int vocab, const void *target,
+                                                      int target_bits, ExpScale k, double tau, dlr_policy p,
+                                                      PolicyOut po, T *out, int64_t out_stride, RowParts w) {
+    __shared__ float coef;
+    const int64_t t = blockIdx.x / w.chunks;
+    const int begin = (int)(blockIdx.x % w.chunks) * w.span, here = vocab - begin < w.span ? vocab - begin : w.span;
+    if (begin && !out) return;
+    const int64_t y = load_target(target, target_bits, t);
+    const float weight = p.weight ? p.weight[t] : 1.f;
+    T *o = out + t * out_stride + begin;
+    if (y < 0 || weight == 0.f) {
+        if (begin == 0 && threadIdx.x == 0) policy_nothing(t, po);
+        if (out) zero_row<T, NT>(o, here);
+        return;
+    }
+    const BlockStat a = join_parts(w, t, k);
+    if (threadIdx.x == 0) {
+        const float zy = y < vocab ? w.zy[t] : __builtin_nanf("");
+        const double lp = target_logprob(zy, a.m, log(a.s), tau);
+        coef = (float)(policy_token(lp, p, t, weight, po, begin == 0) / tau);
+    }
+    if (!out) return;
+    __syncthreads();
+    const float c = coef, neg = (float)(-c / a.s), m = a.m;
+    residual_row<T, NT, 4>(logits + t * stride + begin, o, here, y - begin, c,
+                           [=](float z) { return neg * exp2_hw((z - m) * k.hi); }, false);
 }
 
 // A row held in registers: R packs a thread, pack i of thread x at i NT + x,
@@ -470,10 +574,7 @@ __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t str
     const int64_t y = load_target(target, target_bits, t);
     const float w = p.weight ? p.weight[t] : 1.f;
     if (y < 0 || w == 0.f) {
-        if (threadIdx.x == 0) {
-            po.loss[t] = po.logprob[t] = po.kl[t] = 0.f;
-            po.clipped[t] = 0;
-        }
+        if (threadIdx.x == 0) policy_nothing(t, po);
         if (out) zero_row<T, NT>(out + t * out_stride, vocab);
         return;
     }
@@ -488,7 +589,7 @@ __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t str
     const BlockStat a = join_block<NT>(own, k, lds);
     if (threadIdx.x == 0) {
         const double lp = target_logprob(zy, a.m, log(a.s), tau);
-        coef = (float)(policy_token(lp, p, t, w, po) / tau);
+        coef = (float)(policy_token(lp, p, t, w, po, true) / tau);
     }
     if (!out) return;
     __syncthreads();
@@ -1057,11 +1158,39 @@ static hipError_t by_dtype(int dtype, F f) {
     }
 }
 
+constexpr int64_t kCus = 256;
+
 // Logits of more bytes than the 256 MB Infinity Cache cannot be there when the
 // call begins, nor will a second read find them: they are read past it.
 constexpr int64_t kOnceBytes = INT64_C(1) << 28;
 static bool read_once(const dlr_logits &x) {
     return x.rows * x.vocab * (x.dtype == DLR_DTYPE_F32 ? 4 : 2) > kOnceBytes;
+}
+
+// The chunks of a row: 1, or for few long rows (see RowParts) about two
+// workgroups a CU in all, of 2,048 packs and more.
+static RowParts row_parts(int64_t rows, int64_t vocab, int pack, void *workspace) {
+    const int64_t packs = vocab / pack;
+    int64_t chunks = 1, span = packs;
+    if (rows >= 1 && rows <= 128 && packs >= 8192) {
+        chunks = 2 * kCus / rows < packs / 2048 ? 2 * kCus / rows : packs / 2048;
+        if (chunks > 63) chunks = 63;  // one more where a tail is left over
+        span = (packs + chunks - 1) / chunks;
+        chunks = (vocab + span * pack - 1) / (span * pack);
+    }
+    RowPart *part = static_cast<RowPart *>(workspace);
+    return {part, reinterpret_cast<float *>(part + rows * chunks), (int)chunks, (int)(span * pack)};
+}
+
+int64_t logits_workspace(int64_t rows, int64_t vocab, int32_t dtype) {
+    const RowParts w = row_parts(rows, vocab, dtype == DLR_DTYPE_F32 ? 4 : 8, nullptr);
+    return w.chunks == 1 ? 0 : rows * w.chunks * (int64_t)sizeof(RowPart) + rows * (int64_t)sizeof(float);
+}
+
+template <typename T>
+static hipError_t launch_parts(hipStream_t st, const dlr_logits &x, const float *weight, const RowParts &w) {
+    return launch(k_row_part<T, 512>, x.rows * w.chunks, 512, st, static_cast<const T *>(x.data), x.row_stride,
+                  (int)x.vocab, x.target, x.target_bits, weight, exp_scale(x.temperature), w);
 }
 
 // A row's threads.  Short rows: as few as keep a few packs each, for the
@@ -1075,9 +1204,15 @@ static hipError_t launch_logprob(hipStream_t st, const dlr_logits &x, float *log
                   x.target, x.target_bits, exp_scale(x.temperature), x.temperature, read_once(x), logprob, lse);
 }
 
-hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
+hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, void *workspace, float *logprob, float *lse) {
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
+        const RowParts w = row_parts(x.rows, x.vocab, Pack<T>::N, workspace);
+        if (w.chunks > 1) {
+            const hipError_t r = launch_parts<T>(st, x, nullptr, w);
+            return r != hipSuccess ? r : launch(k_token_finish, x.rows, 64, st, x.target, x.target_bits, (int)x.vocab,
+                                                exp_scale(x.temperature), x.temperature, w, logprob, lse);
+        }
         const int64_t packs = x.vocab / Pack<T>::N;
         if (packs <= 256) return launch_logprob<T, 64>(st, x, logprob, lse);
         if (packs <= 1024) return launch_logprob<T, 128>(st, x, logprob, lse);
@@ -1087,10 +1222,10 @@ hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, float *logp
 
 template <typename T, int NT>
 static hipError_t launch_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad, void *out,
-                              int64_t out_stride) {
-    return launch(k_token_logprob_grad<T, NT>, x.rows, NT, st, static_cast<const T *>(x.data), x.row_stride,
+                              int64_t out_stride, int chunks = 1, int span = 1 << 30) {
+    return launch(k_token_logprob_grad<T, NT>, x.rows * chunks, NT, st, static_cast<const T *>(x.data), x.row_stride,
                   (int)x.vocab, x.target, x.target_bits, x.temperature, read_once(x), lse, grad,
-                  static_cast<T *>(out), out_stride);
+                  static_cast<T *>(out), out_stride, chunks, span);
 }
 
 // As above; rows of 2,048 to 16,384 packs gain from fewer of them in flight
@@ -1101,6 +1236,14 @@ hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const 
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
         const int64_t packs = x.vocab / Pack<T>::N;
+        // Few long rows by chunks of 1,024 packs and more, four workgroups a CU
+        // in all (1 x 131,072 bf16: 2.9 us, 10.6 by one workgroup); not over
+        // the logits, which a chunk may have to read again as a whole.
+        if (x.rows <= kCus && packs >= 2048 && out != x.data) {
+            const int64_t most = 4 * kCus / x.rows < packs / 1024 ? 4 * kCus / x.rows : packs / 1024;
+            const int64_t span = (packs + most - 1) / most * Pack<T>::N, chunks = (x.vocab + span - 1) / span;
+            return launch_grad<T, 512>(st, x, lse, grad, out, out_stride, (int)chunks, (int)span);
+        }
         if (packs <= 256) return launch_grad<T, 64>(st, x, lse, grad, out, out_stride);
         if (packs <= 1024) return launch_grad<T, 128>(st, x, lse, grad, out, out_stride);
         if (packs <= 2048 || packs > 16384) return launch_grad<T, 512>(st, x, lse, grad, out, out_stride);
@@ -1122,11 +1265,19 @@ static hipError_t launch_policy(hipStream_t st, const dlr_logits &x, const dlr_p
 // / 189; 8,000 x 1,000 by 128 / 256: 14 / 18).  Rows longer than a CU's
 // registers hold what fits beside the second reading's own (16 packs a thread
 // spill 16-bit types there: 1,024 x 200,000 386 us, with 8 204).
-hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, float *loss, float *logprob,
-                              float *kl, uint8_t *clipped, void *out, int64_t out_stride) {
+hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, void *workspace, float *loss,
+                              float *logprob, float *kl, uint8_t *clipped, void *out, int64_t out_stride) {
     const PolicyOut po{loss, logprob, kl, clipped};
     return by_dtype(x.dtype, [&](auto e) {
         using T = decltype(e);
+        const RowParts w = row_parts(x.rows, x.vocab, Pack<T>::N, workspace);
+        if (w.chunks > 1) {
+            const hipError_t r = launch_parts<T>(st, x, p.weight, w);
+            return r != hipSuccess ? r : launch(k_policy_finish<T, 512>, x.rows * w.chunks, 512, st,
+                                                static_cast<const T *>(x.data), x.row_stride, (int)x.vocab, x.target,
+                                                x.target_bits, exp_scale(x.temperature), x.temperature, p, po,
+                                                static_cast<T *>(out), out_stride, w);
+        }
         const int64_t packs = x.vocab / Pack<T>::N;
         if (packs <= 512) return launch_policy<T, 128, 4>(st, x, p, po, out, out_stride);
         if (packs <= 1024) return launch_policy<T, 256, 4>(st, x, p, po, out, out_stride);
@@ -1152,8 +1303,6 @@ static bool head_by_dma(const dlr_head &h) {
     return (reinterpret_cast<uintptr_t>(h.head) | reinterpret_cast<uintptr_t>(h.hidden)) % 16 == 0 &&
            h.head_stride % 8 == 0 && h.hidden_stride % 8 == 0 && h.dim % 8 == 0;
 }
-
-constexpr int64_t kCus = 256;
 
 // The workspace: the targets' logits, the picked rows and their count, the
 // tiles' statistics.

@@ -34,9 +34,10 @@ P, i64 = C.c_void_p, C.c_int64
 SYMBOLS = {
     "dlr_losses_last_error": (C.c_char_p,),
     "dlr_losses_runtime": (C.c_char_p,),
-    "dlr_token_logprob": (C.c_int, C.c_int, P, P, P, P),
+    "dlr_logits_workspace": (i64, i64, i64, C.c_int),
+    "dlr_token_logprob": (C.c_int, C.c_int, P, P, P, i64, P, P),
     "dlr_token_logprob_grad": (C.c_int, C.c_int, P, P, P, P, P, i64),
-    "dlr_policy_loss": (C.c_int, C.c_int, P, P, P, P, P, P, P, P, i64),
+    "dlr_policy_loss": (C.c_int, C.c_int, P, P, P, P, i64, P, P, P, P, P, i64),
     "dlr_preference_loss": (C.c_int, C.c_int, P, P, P, P, P, P),
     "dlr_head_logprob_workspace": (i64, i64, i64, i64),
     "dlr_head_logprob": (C.c_int, C.c_int, P, P, P, i64, P, P),
@@ -170,6 +171,15 @@ def _rows(count: int, length: int, like: torch.Tensor):
     return out.unbind(0), out.data_ptr()
 
 
+def _scratch(x: _Logits, like: torch.Tensor):
+    """dlr_logits_workspace's bytes and memory (kept until the launch; the
+    allocator keeps it for the stream).  Most calls need none."""
+    if x.rows > 128 or x.vocab < 32768:
+        return 0, None
+    need = _check(lib.dlr_logits_workspace(x.rows, x.vocab, x.dtype))
+    return need, torch.empty(need, dtype=torch.uint8, device=like.device) if need else None
+
+
 # The current stream of a GPU as an address: torch.cuda.current_stream(gpu).
 # cuda_stream without the Stream object, 2 us of a 10 us call.
 _stream = torch._C._cuda_getCurrentRawStream
@@ -183,7 +193,8 @@ def token_logprob(logits: torch.Tensor, target: torch.Tensor, *,
     (dlr_token_logprob)."""
     gpu, target, x = _logits(logits, target, temperature)
     out, at = _rows(2, x.rows, logits)
-    _check(lib.dlr_token_logprob(gpu, _stream(gpu), C.byref(x), at, at + 4 * x.rows))
+    need, scratch = _scratch(x, logits)
+    _check(lib.dlr_token_logprob(gpu, _stream(gpu), C.byref(x), _ptr(scratch), need, at, at + 4 * x.rows))
     return out
 
 
@@ -231,8 +242,9 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logprob: torch.T
                 kl_coef)
     (loss, logprob, kl), at = _rows(3, rows, logits)
     clipped = torch.empty(rows, dtype=torch.bool, device=logits.device)
-    _check(lib.dlr_policy_loss(gpu, _stream(gpu), C.byref(x), C.byref(p), at, at + 4 * rows, at + 8 * rows,
-                               clipped.data_ptr(), _ptr(dz), 0 if dz is None else dz.stride(0)))
+    need, scratch = _scratch(x, logits)
+    _check(lib.dlr_policy_loss(gpu, _stream(gpu), C.byref(x), C.byref(p), _ptr(scratch), need, at, at + 4 * rows,
+                               at + 8 * rows, clipped.data_ptr(), _ptr(dz), 0 if dz is None else dz.stride(0)))
     return PolicyLoss(loss, logprob, kl, clipped, dz)
 
 

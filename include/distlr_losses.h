@@ -15,9 +15,11 @@
  *     of that device; NULL: its default stream) and the call returns without
  *     waiting.  Calls may be captured into a graph.  The calling thread's
  *     current device is unchanged on return.
- *   - Scratch memory is the caller's (dlr_head_logprob_workspace): two calls
+ *   - Scratch memory is the caller's (dlr_logits_workspace,
+ *     dlr_head_logprob_workspace; 256-byte aligned device memory, not
+ *     initialised, free for other use once the call's work is done): two calls
  *     that may run at the same time, or two captured graphs that do, need two
- *     workspaces.  No other call uses any.
+ *     workspaces.
  *   - Rows: `data` (the hidden states, the weights) is row-major with
  *     contiguous elements in a row; rows start row_stride elements apart, at
  *     any alignment of the element type.
@@ -75,9 +77,15 @@ typedef struct dlr_logits {
     double temperature;     /* 1e-6 .. 1e6                                    */
 } dlr_logits;
 
+/* Bytes of the scratch memory of dlr_token_logprob and dlr_policy_loss, or < 0:
+ * 0 (then the workspace may be NULL) but for few long rows, at most 128 of
+ * 32,768 classes and more, whose chunks meet there. */
+int64_t dlr_logits_workspace(int64_t rows, int64_t vocab, int dtype);
+
 /* lse[t] = log sum_j exp(z_tj / temperature), logprob[t] = z_ty / temperature
  * - lse[t], y = target[t].  Each logit is read once. */
-int dlr_token_logprob(int device, void *stream, const dlr_logits *x, float *logprob, float *lse);
+int dlr_token_logprob(int device, void *stream, const dlr_logits *x, void *workspace, int64_t workspace_bytes,
+                      float *logprob, float *lse);
 
 /* The gradient of sum_t grad[t] * logprob[t] with respect to the logits (the
  * softmax residual): grad_logits[t][j] = grad[t] / temperature * (1[j = y] -
@@ -95,8 +103,8 @@ int dlr_token_logprob_grad(int device, void *stream, const dlr_logits *x, const 
  *   loss[t] = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef kl
  * The objective is sum_t weight[t] * loss[t]; grad_logits is its gradient.
  * A row of weight 0 takes no part (like a negative target).  clipped[t] = 1
- * where the clip holds the surrogate (its gradient is 0 there).  One pass:
- * logits to gradient in one launch. */
+ * where the clip holds the surrogate (its gradient is 0 there).  One pass over
+ * the logits, which are read once where a row fits a CU's registers. */
 typedef struct dlr_policy {
     const float *old_logprob;   /* rows                                       */
     const float *ref_logprob;   /* rows; NULL: no KL term (kl_coef must be 0) */
@@ -108,8 +116,9 @@ typedef struct dlr_policy {
 } dlr_policy;
 /* loss, logprob, kl, clipped: rows each.  grad_logits: NULL for no gradient,
  * else as for dlr_token_logprob_grad (x->data itself is allowed). */
-int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_policy *p, float *loss, float *logprob,
-                    float *kl, uint8_t *clipped, void *grad_logits, int64_t grad_row_stride);
+int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_policy *p, void *workspace,
+                    int64_t workspace_bytes, float *loss, float *logprob, float *kl, uint8_t *clipped,
+                    void *grad_logits, int64_t grad_row_stride);
 
 /* The paired logistic (preference) loss over packed ragged sequences.
  * Sequence i is tokens [offsets[i], offsets[i+1]); sequences 0 .. pairs-1
@@ -155,8 +164,7 @@ typedef struct dlr_head {
     int32_t target_bits;
     double temperature;
 } dlr_head;
-/* Bytes of dlr_head_logprob's workspace (256-byte aligned device memory), or
- * < 0. */
+/* Bytes of dlr_head_logprob's scratch memory, or < 0. */
 int64_t dlr_head_logprob_workspace(int64_t rows, int64_t vocab, int64_t dim);
 int dlr_head_logprob(int device, void *stream, const dlr_head *h, void *workspace, int64_t workspace_bytes,
                      float *logprob, float *lse);

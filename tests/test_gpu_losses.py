@@ -100,7 +100,8 @@ def check_grad(got, z, y, coef, coef_err, temperature, extra=0.0, lse=None):
 
 
 SHAPES = [(1, 1, 0), (3, 1, 3), (2, 2, 0), (5, 7, 1), (4, 8, 0), (3, 9, 2), (1, 511, 0), (3, 513, 5), (17, 1000, 0),
-          (2, 4097, 7), (3, 16389, 0), (2, 50257, 47), (260, 129, 0), (1, 131075, 0)]
+          (2, 4097, 7), (3, 16389, 0), (2, 50257, 47), (260, 129, 0), (1, 131075, 0), (5, 262147, 3),
+          (100, 65541, 1)]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
@@ -219,7 +220,7 @@ def test_policy_loss(L, rows, vocab, pad, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("vocab", [5, 700, 4100, 40001])
+@pytest.mark.parametrize("vocab", [5, 700, 4100, 40001, 140003])
 def test_masked_classes_infinities_and_nan(L, dtype, vocab):
     inf, nan = float("inf"), float("nan")
     rows = 8
@@ -718,7 +719,7 @@ def test_the_current_device_and_the_last_error_stay(L, dlr):
     z, y = torch.zeros(3, 5).cuda(), torch.zeros(3, dtype=torch.int64).cuda()
     x = L._logits(z, y, 1.0)[2]
     import ctypes
-    assert L.lib.dlr_token_logprob(99, None, ctypes.byref(x), z.data_ptr(), z.data_ptr()) == -4
+    assert L.lib.dlr_token_logprob(99, None, ctypes.byref(x), None, 0, z.data_ptr(), z.data_ptr()) == -4
     assert torch.cuda.current_device() == 0
     torch.cuda.synchronize()  # the failed call's error is not reported again
     lp, _ = L.token_logprob(z, y)

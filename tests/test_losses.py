@@ -78,9 +78,9 @@ BAD_LOGITS = [
 @pytest.mark.parametrize("kw,word", BAD_LOGITS, ids=lambda v: str(v)[:40])
 def test_bad_logits_are_refused_by_every_call(kw, word):
     x, p = logits(**kw), L._Policy(D, None, D, None, 0.2, 0.2, 0.0)
-    for rc in (L.lib.dlr_token_logprob(0, None, C.byref(x), D, E),
+    for rc in (L.lib.dlr_token_logprob(0, None, C.byref(x), None, 0, D, E),
                L.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, D, E, 8),
-               L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, E, None, 0)):
+               L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, 0, E, E, E, E, None, 0)):
         rc, msg = code(rc)
         assert rc == dlr.E_ARG and word in msg
 
@@ -88,16 +88,16 @@ def test_bad_logits_are_refused_by_every_call(kw, word):
 def test_null_descriptors_and_outputs():
     x, p = logits(), L._Policy(D, None, D, None, 0.2, 0.2, 0.0)
     calls = [
-        lambda: L.lib.dlr_token_logprob(0, None, None, D, E),
-        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), None, E),
-        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), D, None),
-        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), D + 2, E),
+        lambda: L.lib.dlr_token_logprob(0, None, None, None, 0, D, E),
+        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), None, 0, None, E),
+        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), None, 0, D, None),
+        lambda: L.lib.dlr_token_logprob(0, None, C.byref(x), None, 0, D + 2, E),
         lambda: L.lib.dlr_token_logprob_grad(0, None, C.byref(x), None, D, E, 8),
         lambda: L.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, None, E, 8),
         lambda: L.lib.dlr_token_logprob_grad(0, None, C.byref(x), D, D, None, 8),
-        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), None, E, E, E, E, None, 0),
-        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, E, E, E, None, 0),
-        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, None, None, 0),
+        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), None, None, 0, E, E, E, E, None, 0),
+        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, 0, None, E, E, E, None, 0),
+        lambda: L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, 0, E, E, E, None, None, 0),
         lambda: L.lib.dlr_preference_loss(0, None, None, E, E, E, None),
         lambda: L.lib.dlr_head_logprob(0, None, None, D, 1 << 20, E, E),
     ]
@@ -111,7 +111,7 @@ def test_null_descriptors_and_outputs():
 def test_gradients_that_do_not_fit(grad, stride, word):
     x, p = logits(), L._Policy(E, None, E, None, 0.2, 0.2, 0.0)
     for rc in (L.lib.dlr_token_logprob_grad(0, None, C.byref(x), E, E, grad, stride),
-               L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), F, F, F, F, grad, stride)):
+               L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, 0, F, F, F, F, grad, stride)):
         rc, msg = code(rc)
         assert rc == dlr.E_ARG and word in msg
 
@@ -131,7 +131,7 @@ def test_bad_policy(kw, word):
     v = dict(old_logprob=D, ref_logprob=D, advantage=D, weight=None, clip_low=0.2, clip_high=0.2, kl_coef=0.1)
     v.update(kw)
     x, p = logits(), L._Policy(**v)
-    rc, msg = code(L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), E, E, E, E, None, 0))
+    rc, msg = code(L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, 0, E, E, E, E, None, 0))
     assert rc == dlr.E_ARG and word in msg
 
 
@@ -181,13 +181,30 @@ def test_head_workspace():
         assert rc == dlr.E_ARG and "workspace" in msg
 
 
+def test_logits_workspace():
+    size = L.lib.dlr_logits_workspace
+    assert size(1, 32000, L.DTYPE_BF16) == 0 and size(129, 1 << 20, L.DTYPE_F32) == 0 and size(0, 1 << 20, 0) == 0
+    for rows, vocab, dtype in ((0, 0, 0), (-1, 9, 0), (4, (1 << 30) + 1, 0), (4, 100, 3)):
+        assert code(size(rows, vocab, dtype))[0] == dlr.E_ARG
+    need = size(4, 200000, L.DTYPE_BF16)
+    assert need > 0
+    assert all(size(r, v, d) == 0 for r in (1, 128) for v in (1, 32767) for d in range(3))  # what the binding skips
+    x = logits(rows=4, vocab=200000, row_stride=200000, dtype=L.DTYPE_BF16)
+    p = L._Policy(D, None, D, None, 0.2, 0.2, 0.0)
+    for ws, n in ((None, need), (E, need - 1), (E + 4, need)):
+        for rc in (L.lib.dlr_token_logprob(0, None, C.byref(x), ws, n, D, E),
+                   L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), ws, n, D, D, D, D, None, 0)):
+            rc, msg = code(rc)
+            assert rc == dlr.E_ARG and "workspace" in msg
+
+
 def test_a_device_that_is_not_there():
     x, p = logits(), L._Policy(D, None, D, None, 0.2, 0.2, 0.0)
     q = L._Preference(A, None, None, B, None, 2, 10, 0.1, 0.0, 0.0, 0, 0)
     h = L._Head(A, A, B, 4, 100, 64, 64, 64, L.DTYPE_BF16, 64, 1.0)
-    for rc in (L.lib.dlr_token_logprob(99, None, C.byref(x), D, E),
+    for rc in (L.lib.dlr_token_logprob(99, None, C.byref(x), None, 0, D, E),
                L.lib.dlr_token_logprob_grad(99, None, C.byref(x), D, D, E, 8),
-               L.lib.dlr_policy_loss(99, None, C.byref(x), C.byref(p), E, E, E, E, None, 0),
+               L.lib.dlr_policy_loss(99, None, C.byref(x), C.byref(p), None, 0, E, E, E, E, None, 0),
                L.lib.dlr_preference_loss(99, None, C.byref(q), D, D, D, E),
                L.lib.dlr_head_logprob(99, None, C.byref(h), D, 1 << 20, E, E)):
         assert code(rc)[0] == -4  # DLR_E_HIP
@@ -195,9 +212,9 @@ def test_a_device_that_is_not_there():
 
 def test_no_rows_is_a_valid_call():
     x, p = logits(rows=0, data=None, target=None), L._Policy(None, None, None, None, 0.2, 0.2, 0.0)
-    assert L.lib.dlr_token_logprob(0, None, C.byref(x), None, None) == 0
+    assert L.lib.dlr_token_logprob(0, None, C.byref(x), None, 0, None, None) == 0
     assert L.lib.dlr_token_logprob_grad(0, None, C.byref(x), None, None, None, 0) == 0
-    assert L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, None, None, None, None, 0) == 0
+    assert L.lib.dlr_policy_loss(0, None, C.byref(x), C.byref(p), None, 0, None, None, None, None, None, 0) == 0
     q = L._Preference(None, None, None, None, None, 0, 0, 0.1, 0.0, 0.0, 0, 0)
     assert L.lib.dlr_preference_loss(0, None, C.byref(q), None, None, None, None) == 0
     h = L._Head(None, None, None, 0, 100, 64, 64, 64, L.DTYPE_BF16, 64, 1.0)
