@@ -880,9 +880,9 @@ __global__ __launch_bounds__(1024) void k_head_pick(const void *target, int targ
 #define SCHED_LDS(n) __builtin_amdgcn_sched_group_barrier(256, n, 0)
 
 // Measured (bf16): 256 x 256 tiles, 8 waves of 128 x 64, 4096 x 4096 x 65536
-// 1.59 ms, 1,380 TFLOP/s, softmax included, where the library's product alone
-// takes 1.54; the matrix cores are busy 60% of the time at 2.0 GHz and LDS
-// reads about as long.  4 waves of 128 x 128 read a third less from LDS, but
+// 1.57 ms, 1,400 TFLOP/s, softmax included, where the library's product alone
+// takes 1.54; the matrix cores are busy 75% of the cycles, at the 1.8 GHz that
+// they leave of the clock.  4 waves of 128 x 128 read a third less from LDS, but
 // the compiler then moves accumulators between register files (994 TFLOP/s);
 // 32 x 32 products meet LDS banks twice in this layout (1,109); a workgroup
 // that goes on to its next tile and fetches it under this one's end spills
@@ -1077,6 +1077,140 @@ __global__ __launch_bounds__(WV *WT * 64) void k_head_dma(dlr_head h, int64_t v_
             for (int w = 1; w < WV; ++w) a = join(a, stat[w * TT + i], k);
             part[vt * h.rows + t0 + i] = make_float2(a.m, a.s);
         }
+}
+
+// ---- small tiles: the dimension split over a workgroup's four waves
+//
+// A tile of TV = MV * 16 classes x TT = MT * 16 tokens keeps one wave too little
+// busy to hide a stage's barrier and LDS trips, and few classes leave most CUs
+// without a tile.  So the four waves take every fourth stage each, from LDS
+// rings of their own: no barrier until their products are added, in a fixed
+// order.
+template <typename T, int MV, int MT, int S>
+__global__ __launch_bounds__(256) void k_head_waves(dlr_head h, int64_t v_first, HeadPick pick, float2 *part,
+                                                    float *zy) {
+    constexpr int TV = MV * 16, TT = MT * 16, kRow = 128, L = (TV + TT) / 8, B = MV * MT / 4;
+    static_assert(MV == 4 && (MT == 1 || MT == 4) && S >= 2 && L * (S - 1) < 64, "a wave's share of the blocks");
+    __shared__ __attribute__((aligned(256))) char sm[4][S][(TV + TT) * kRow];
+    __shared__ RowStat stat[4][TT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t used = pick.row ? *pick.count : h.rows;
+    const int64_t vtiles = (h.vocab - v_first + TV - 1) / TV, ttiles = (used + TT - 1) / TT;
+    if (blockIdx.x >= vtiles * ttiles) return;  // the launch counts all rows
+    const int64_t vt = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / ttiles)), v0 = v_first + vt * TV;
+    const int64_t t0 = (int64_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x % ttiles)) * TT;
+    const int dim = (int)h.dim, steps = (dim + 63) / 64;
+    auto token = [&](int64_t t) { return pick.row ? (int64_t)pick.row[t] : t; };
+
+    const char *src[L];  // this lane's places in the wave's DMA loads, of the wave's next stage
+    const int chunk = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+    for (int q = 0; q < L; ++q) {
+        const bool x = q >= TV / 8;
+        const int r = (x ? q - TV / 8 : q) * 8 + (lane >> 3);
+        const int64_t first = x ? t0 : v0, last = (x ? used : h.vocab) - 1;
+        int64_t at = first + r < last ? first + r : last;
+        if (x) at = token(at);
+        src[q] = static_cast<const char *>(x ? h.hidden : h.head) + at * (x ? h.hidden_stride : h.head_stride) * 2 +
+                 chunk * 16 + wave * 128;
+    }
+    auto fill = [&](int step, int buf) {  // dim is a multiple of 8: zeros behind it
+        const bool in = step * 64 + chunk * 8 < dim;
+#pragma unroll
+        for (int q = 0; q < L; ++q) {
+            lds_dma16(in ? src[q] : (const char *)&kZero16, sm[wave][buf] + q * 1024);
+            src[q] += 4 * 128;
+        }
+    };
+    const int at = (lane & 15) * kRow;
+    f32x4 acc[MV][MT] = {};
+    int buf = 0;
+#pragma unroll
+    for (int p = 0; p < S; ++p)
+        if (wave + 4 * p < steps) fill(wave + 4 * p, p);
+    for (int step = wave; step < steps; step += 4) {
+        // this stage has landed; the ring's others stay in flight
+        if (step + 4 * (S - 1) < steps)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L *(S - 1)) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const char *sv = sm[wave][buf] + at, *sx = sv + TV * kRow;
+        u32x4 a[2][MV], b[2][MT];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int slot = ((half * 4 + (lane >> 4)) ^ (lane & 7)) * 16;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) b[half][j] = *reinterpret_cast<const u32x4 *>(sx + j * 16 * kRow + slot);
+#pragma unroll
+            for (int i = 0; i < MV; ++i) a[half][i] = *reinterpret_cast<const u32x4 *>(sv + i * 16 * kRow + slot);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the slot is free
+        if (step + 4 * S < steps) fill(step + 4 * S, buf);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < MV; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) acc[i][j] = mfma(a[half][i], b[half][j], acc[i][j], T());
+        buf = buf + 1 < S ? buf + 1 : 0;
+    }
+    // the waves' products added; wave w then has blocks w B .. w B + B - 1 of
+    // the tile's MV x MT, counted along the classes
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    f32x4 *sum = reinterpret_cast<f32x4 *>(sm);  // [4][MV * MT][64]
+    static_assert(sizeof(f32x4) * 4 * MV * MT * 64 <= sizeof sm, "they fit");
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int i = 0; i < MV; ++i) sum[(wave * MV * MT + j * MV + i) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    const ExpScale k = exp_scale(h.temperature);
+    const int classes = h.vocab - v0 < TV ? (int)(h.vocab - v0) : TV;
+    const int first = wave * B, j = first / MV;
+    const int64_t t = t0 + j * 16 + (lane & 15);
+    const int64_t row = t < used ? token(t) : -1;
+    const int64_t y = (row >= 0 ? load_target(h.target, h.target_bits, row) : -1) - v0;
+    const int target = y >= 0 && y < TV ? (int)y : -1;  // in the tile
+    f32x4 z[B];
+    float m = NEG_INF;
+#pragma unroll
+    for (int n = 0; n < B; ++n) {
+        z[n] = sum[(first + n) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) z[n] += sum[(w * MV * MT + first + n) * 64 + lane];
+        const int base = ((first + n) % MV) * 16 + (lane >> 4) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (base + e >= classes) z[n][e] = NEG_INF;
+            if (base + e == target) zy[row] = z[n][e];
+            m = fmaxf(m, z[n][e]);
+        }
+    }
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float r = m == NEG_INF ? 0.f : m;
+    float s[B];
+#pragma unroll
+    for (int n = 0; n < B; ++n) {
+        float e4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) e4[e] = exp2_scaled(z[n][e] - r, k);
+        s[n] = tree_sum(e4);
+    }
+    float total = tree_sum(s);
+    total += __shfl_xor(total, 16);
+    total += __shfl_xor(total, 32);
+    constexpr int W = B >= MV ? 1 : 4;  // waves that share a token
+    if (lane < 16) stat[W == 1 ? 0 : wave][j * 16 + lane] = {m, total};
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (i < TT && t0 + i < used) {
+        RowStat q = stat[0][i];
+#pragma unroll
+        for (int w = 1; w < W; ++w) q = join(q, stat[w][i], k);
+        part[vt * h.rows + t0 + i] = make_float2(q.m, q.s);
+    }
 }
 
 // The tiles' statistics, joined: RT tokens a workgroup (their statistics lie
@@ -1338,6 +1472,16 @@ static hipError_t launch_head_dma(hipStream_t st, dlr_head h, int64_t first, int
     return launch(k_head_dma<T, WV, WT, MV, MT, S>, vtiles * ttiles, WV * WT * 64, st, h, first, pick, part, w.zy);
 }
 
+template <typename T, int MT, int S>
+static hipError_t launch_head_waves(hipStream_t st, dlr_head h, int64_t first, int64_t end, const HeadPick &pick,
+                                    const HeadSpace &w, int64_t &tiles) {
+    const int64_t vtiles = (end - first + 63) / 64, ttiles = (h.rows + MT * 16 - 1) / (MT * 16);
+    h.vocab = end;
+    float2 *part = w.part + tiles * h.rows;
+    tiles += vtiles;
+    return launch(k_head_waves<T, 4, MT, S>, vtiles * ttiles, 256, st, h, first, pick, part, w.zy);
+}
+
 // The tiles of more than 16 rows.  What a tile costs: microseconds per stage
 // of 64, alone on its CU or two of them on it, measured from 1 x 8 to 32,768
 // tiles at dim 512 and 4096; and per round of the CUs its ends.
@@ -1396,6 +1540,11 @@ static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t dim) {
     return plan;
 }
 
+// Up to this many tiles of 64 classes they go by k_head_waves (1 x 8192 x 1000:
+// 18 us against 24, 100 x 8192 x 1500 31 against 42), beyond by k_head_dma, two
+// workgroups a CU (300 x 4096 x 3000: 28 against 30).
+constexpr int64_t kFewTiles = 128;
+
 // Up to 16 rows the head's bytes are all there is: 256 classes a workgroup once
 // that is most of two workgroups a CU, else 64 with a deeper queue (1 row x
 // 4096: 131,072 classes 180 us against 190, 65,536 classes 118 against 105).
@@ -1419,6 +1568,8 @@ static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const Hea
         tiles = (h.vocab + kTileV - 1) / kTileV;
         return launch(k_head_tile<T>, tiles * ((h.rows + kTileT - 1) / kTileT), 256, st, h, w.part, w.zy);
     }
+    if (h.rows <= 16 && tiles_of(h.vocab, 64) <= kFewTiles)
+        return launch_head_waves<T, 1, 2>(st, h, 0, h.vocab, pick, w, tiles);
     if (h.rows <= 16)
         return few_rows_tile(h.vocab) == 256 ? launch_head_dma<T, 8, 1, 2, 1, 2>(st, h, 0, h.vocab, pick, w, tiles)
                                          : launch_head_dma<T, 4, 1, 1, 1, 4>(st, h, 0, h.vocab, pick, w, tiles);
@@ -1427,7 +1578,10 @@ static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const Hea
             case 0: return launch_head_dma<T, 2, 4, 8, 4, 2>(st, h, first, end, pick, w, tiles);
             case 1: return launch_head_dma<T, 4, 2, 4, 4, 3>(st, h, first, end, pick, w, tiles);
             case 2: return launch_head_dma<T, 4, 1, 2, 4, 3>(st, h, first, end, pick, w, tiles);
-            default: return launch_head_dma<T, 4, 1, 1, 4, 4>(st, h, first, end, pick, w, tiles);
+            default:
+                return tiles_of(end - first, 64) * tiles_of(h.rows, 64) <= kFewTiles
+                           ? launch_head_waves<T, 4, 2>(st, h, first, end, pick, w, tiles)
+                           : launch_head_dma<T, 4, 1, 1, 4, 4>(st, h, first, end, pick, w, tiles);
         }
     };
     const HeadPlan plan = head_plan(h.rows, h.vocab, h.dim);

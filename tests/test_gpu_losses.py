@@ -423,7 +423,8 @@ def test_preference_bad_offsets_and_no_pairs(L):
 # ------------------------------------------------------------------------ head
 
 HEAD_SHAPES = [(1, 1, 1), (1, 300, 64), (2, 129, 8), (3, 128, 72), (16, 1000, 256), (17, 513, 200), (33, 257, 33),
-               (65, 1025, 129), (130, 300, 520), (129, 128, 31), (257, 700, 64), (5, 5003, 1024), (300, 391, 96)]
+               (65, 1025, 129), (130, 300, 520), (129, 128, 31), (257, 700, 64), (5, 5003, 1024), (300, 391, 96), (16, 9000, 72),
+               (64, 64, 320), (100, 1100, 1000), (90, 9001, 136), (7, 77, 1016)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
