@@ -617,7 +617,7 @@ typedef uint32_t u32_any __attribute__((aligned(1)));
 // the pair's one slope written over its tokens.  4 tokens a thread and step,
 // loaded whether the mask counts them or not: a load that waits for its mask
 // costs a second trip to memory.  Bound by latency, three dependent trips and
-// the logarithms: 1,024 pairs of 1.5M tokens 9 us (19.6 a token at a time
+// the logarithms: 1,024 pairs of 1.5M tokens 11 us (19.6 a token at a time
 // behind its mask), two pairs 4.  One workgroup a pair also where the
 // sequences are very long (1 x 400,000 tokens 69 us): the logits of such a
 // pair take a thousand times as long.
@@ -1426,9 +1426,13 @@ hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float
                                   float *rejected, float *grad) {
     const int64_t blocks = p.pairs ? p.pairs : 1;
     const PairOut o{loss, chosen, rejected, grad};
-    // 2 x 4 tokens a thread on average; a large workgroup only for long sequences
-    return p.tokens / blocks > 2048 ? launch(k_preference_loss<1024>, blocks, 1024, st, p, o)
-                                    : launch(k_preference_loss<256>, blocks, 256, st, p, o);
+    // A large workgroup for long sequences, where there are CUs for it (us by
+    // 256 / 512 / 1,024 threads: 16 pairs of 1,000 tokens 5.7 / 4.7 / 5.3, 1,024
+    // of 1,465 11 / 12 / 19, 64 of 23,400 - / 30 / 23).
+    const int64_t each = p.tokens / blocks;
+    if (each > 8192) return launch(k_preference_loss<1024>, blocks, 1024, st, p, o);
+    if (each > 512 && blocks <= 2 * kCus) return launch(k_preference_loss<512>, blocks, 512, st, p, o);
+    return launch(k_preference_loss<256>, blocks, 256, st, p, o);
 }
 
 // Whether the rows can go through the DMA kernels: 16-byte chunks of rows that
