@@ -27,8 +27,8 @@ class DeviceScope {
         if (err_ == hipSuccess && before_ != device) {
             err_ = hipSetDevice(device);
             set_ = err_ == hipSuccess;
-            if (!set_) (void)hipGetLastError();  // reported here, not by the caller's next call
         }
+        if (err_ != hipSuccess) (void)hipGetLastError();  // reported here, not by the caller's next call
     }
     ~DeviceScope() {
         if (set_) (void)hipSetDevice(before_);

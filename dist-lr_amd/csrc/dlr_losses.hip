@@ -701,7 +701,8 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     if (bad) u = reward[0] = reward[1] = __builtin_nan("");
     const double w = p.weight ? (double)p.weight[pair] : 1.0;
     if (threadIdx.x == 0) {
-        o.loss[pair] = (float)((1.0 - eps) * softplus(-u) + eps * softplus(u));
+        // a side without weight adds nothing, also where it is infinite
+        o.loss[pair] = (float)((eps < 1.0 ? (1.0 - eps) * softplus(-u) : 0.0) + (eps > 0.0 ? eps * softplus(u) : 0.0));
         o.chosen[pair] = (float)reward[0];
         o.rejected[pair] = (float)reward[1];
     }

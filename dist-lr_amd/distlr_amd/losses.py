@@ -1,6 +1,8 @@
-"""Softmax losses on torch tensors (include/distlr_losses.h): log-probabilities of given classes and their gradient,
-the paired logistic (preference) loss, the clipped policy loss, and
-log-probabilities straight from hidden states and the output layer's weights.
+"""Softmax losses on torch tensors (include/distlr_losses.h).
+
+Log-probabilities of given classes and their gradient, the paired logistic
+(preference) loss, the clipped policy loss, and log-probabilities straight
+from hidden states and the output layer's weights.
 
 The many-class counterparts of the engine's margin, residual and log-loss
 (lr.cc:35-40, 47-63).  Like the engine they return gradients, they do not

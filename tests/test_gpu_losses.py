@@ -813,3 +813,18 @@ def test_autograd_notices_a_gradient_written_over_the_logits(L):
     L.token_logprob_grad(h.detach(), y, lse, torch.ones(4).cuda(), out=h.detach())
     with pytest.raises(RuntimeError):
         loss.backward()
+
+
+def test_preference_with_an_impossible_sequence(L):
+    # a token of probability 0 in the sequence that is not preferred: u = inf, loss 0, nothing flows back
+    inf = float("inf")
+    off = torch.tensor([0, 2, 4]).cuda()
+    worse = torch.tensor([-1.0, -2.0, -inf, -1.0]).cuda()
+    out = L.preference_loss(worse, None, off, beta=0.5)
+    assert out.loss[0] == 0 and out.rejected_reward[0] == -inf and (out.grad == 0).all()
+    out = L.preference_loss(-worse.flip(0) * -1, None, off, beta=0.5)  # in the preferred one: loss inf, slope -1
+    assert out.loss[0] == inf and torch.equal(out.grad.cpu(), torch.tensor([-0.5, -0.5, 0.5, 0.5]))
+    out = L.preference_loss(worse, None, off, beta=0.5, label_smoothing=0.1)
+    assert out.loss[0] == inf
+    out = L.preference_loss(worse, None, off, beta=0.5, label_smoothing=1.0)  # all weight on the other side
+    assert out.loss[0] == inf
