@@ -1494,7 +1494,8 @@ struct HeadTile {
     int64_t tv, tt;
     double alone, two;  // two 0: one workgroup a CU
 };
-constexpr HeadTile kHeadTiles[] = {{256, 256, 1.56, 0}, {256, 128, 0.9, 0}, {128, 64, 0.42, 0.67}, {64, 64, 0.3, 0.55}};
+constexpr HeadTile kHeadTiles[] = {
+    {256, 256, 1.56, 0}, {256, 192, 1.2, 0}, {256, 128, 0.9, 0}, {128, 64, 0.42, 0.67}, {64, 64, 0.3, 0.55}};
 constexpr double kEnds = 3, kLaunch = 3;
 
 static int64_t tiles_of(int64_t classes, int64_t tv) { return (classes + tv - 1) / tv; }
@@ -1514,14 +1515,14 @@ struct HeadPlan {
 
 // The cheapest tile for all classes, or a large one for as many classes as
 // fill whole rounds of the CUs and the cheapest for the others: 333 x 1536 x
-// 50257 is 2.3 rounds of 256 x 128 tiles, paid as 3 (74 us), or one round of
-// 256 x 256 tiles and one of 256 x 128 (71).  200 x 4096 x 32000: 63 us by 256
+// 50257 is 2.3 rounds of 256 x 128 tiles, paid as 3 (82 us), or one round of
+// 256 x 192 tiles and one of 256 x 128 (73).  200 x 4096 x 32000: 63 us by 256
 // x 128, 95 by 256 x 256; 2048 x 4096 x 1000: 30 us by 128 x 64, 81.
 static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t dim) {
     const int64_t stages = (dim + 63) / 64;
     auto best = [&](int64_t classes) {
         int i = 0;
-        for (int j = 1; j < 4; ++j)
+        for (int j = 1; j < 5; ++j)
             if (head_cost(kHeadTiles[j], rows, classes, stages) < head_cost(kHeadTiles[i], rows, classes, stages))
                 i = j;
         return i;
@@ -1529,7 +1530,7 @@ static HeadPlan head_plan(int64_t rows, int64_t vocab, int64_t dim) {
     const int whole = best(vocab);
     HeadPlan plan{whole, whole, vocab};
     double cost = head_cost(kHeadTiles[whole], rows, vocab, stages);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 3; ++i) {
         const HeadTile &t = kHeadTiles[i];
         const int64_t ttiles = (rows + t.tt - 1) / t.tt, rounds = vocab / t.tv * ttiles / kCus;
         const int64_t classes = rounds * kCus / ttiles * t.tv;
@@ -1581,8 +1582,9 @@ static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const Hea
     auto by = [&](int tile, int64_t first, int64_t end) {
         switch (tile) {
             case 0: return launch_head_dma<T, 2, 4, 8, 4, 2>(st, h, first, end, pick, w, tiles);
-            case 1: return launch_head_dma<T, 4, 2, 4, 4, 3>(st, h, first, end, pick, w, tiles);
-            case 2: return launch_head_dma<T, 4, 1, 2, 4, 3>(st, h, first, end, pick, w, tiles);
+            case 1: return launch_head_dma<T, 2, 4, 8, 3, 2>(st, h, first, end, pick, w, tiles);
+            case 2: return launch_head_dma<T, 4, 2, 4, 4, 3>(st, h, first, end, pick, w, tiles);
+            case 3: return launch_head_dma<T, 4, 1, 2, 4, 3>(st, h, first, end, pick, w, tiles);
             default:
                 return tiles_of(end - first, 64) * tiles_of(h.rows, 64) <= kFewTiles
                            ? launch_head_waves<T, 4, 2>(st, h, first, end, pick, w, tiles)
