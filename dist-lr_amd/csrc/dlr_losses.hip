@@ -493,13 +493,14 @@ __global__ __launch_bounds__(NT) void k_policy_finish(const T *logits, int64_t s
                            [=](float z) { return neg * exp2_hw((z - m) * k.hi); }, false);
 }
 
-// A row held in registers: R packs a thread, pack i of thread x at i NT + x,
-// and the element of the tail that is this thread's.
-template <typename T, int NT, int R>
+// A row held by its workgroup: R packs a thread in registers, Q in LDS, pack i
+// of thread x at i NT + x, and the element of the tail that is this thread's.
+template <typename T, int NT, int R, int Q>
 struct HeldRow {
     using PK = Pack<T>;
     u32x4 v[R];
     float tail;
+    u32x4 *lds;  // [Q][NT], a thread touches its own
 
     __device__ void load(const T *row, int vocab, bool once) {
         const int packs = vocab / PK::N;
@@ -510,6 +511,21 @@ struct HeldRow {
         }
         const int at = packs * PK::N + threadIdx.x;
         tail = at < vocab ? (float)row[at] : NEG_INF;
+        constexpr int G = 3;
+#pragma unroll
+        for (int i = 0; i < Q; i += G) {
+            u32x4 w[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int p = (R + i + g) * NT + threadIdx.x;
+                if (i + g < Q && p < packs) w[g] = load_pack(row, p, once);
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int p = (R + i + g) * NT + threadIdx.x;
+                if (i + g < Q && p < packs) lds[(i + g) * NT + threadIdx.x] = w[g];
+            }
+        }
     }
     __device__ RowStat stat(int vocab, ExpScale k) const {
         const int packs = vocab / PK::N;
@@ -519,6 +535,13 @@ struct HeldRow {
             if (i * NT + (int)threadIdx.x < packs) {
 #pragma unroll
                 for (int e = 0; e < PK::N; ++e) m = fmaxf(m, PK::get(v[i], e));
+            }
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+            if ((R + i) * NT + (int)threadIdx.x < packs) {
+                const u32x4 w = lds[i * NT + threadIdx.x];
+#pragma unroll
+                for (int e = 0; e < PK::N; ++e) m = fmaxf(m, PK::get(w, e));
             }
         const float r = m == NEG_INF ? 0.f : m;
         float s[R];
@@ -532,7 +555,28 @@ struct HeldRow {
                 s[i] = tree_sum(x);
             }
         }
-        return {m, tree_sum(s) + exp2_scaled(tail - r, k)};
+        float total = tree_sum(s) + exp2_scaled(tail - r, k);
+        for (int i = 0; i < Q; ++i)
+            if ((R + i) * NT + (int)threadIdx.x < packs) {
+                const u32x4 w = lds[i * NT + threadIdx.x];
+                float x[PK::N];
+#pragma unroll
+                for (int e = 0; e < PK::N; ++e) x[e] = exp2_scaled(PK::get(w, e) - r, k);
+                total += tree_sum(x);
+            }
+        return {m, total};
+    }
+    template <typename F>
+    static __device__ void write(T *out, int p, const u32x4 &v, int64_t y, float c, F prob) {
+        float f[PK::N];
+#pragma unroll
+        for (int e = 0; e < PK::N; ++e) f[e] = prob(PK::get(v, e));
+        const int64_t at = y - (int64_t)p * PK::N;
+        if (at >= 0 && at < PK::N) {
+#pragma unroll
+            for (int e = 0; e < PK::N; ++e) f[e] += e == at ? c : 0.f;
+        }
+        store_pack(out, p, PK::put(f));
     }
     template <typename F>
     __device__ void residual(T *out, int vocab, int64_t y, float c, F prob) const {
@@ -540,16 +584,11 @@ struct HeldRow {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int p = i * NT + threadIdx.x;
-            if (p >= packs) continue;
-            float f[PK::N];
-#pragma unroll
-            for (int e = 0; e < PK::N; ++e) f[e] = prob(PK::get(v[i], e));
-            const int64_t at = y - (int64_t)p * PK::N;
-            if (at >= 0 && at < PK::N) {
-#pragma unroll
-                for (int e = 0; e < PK::N; ++e) f[e] += e == at ? c : 0.f;
-            }
-            store_pack(out, p, PK::put(f));
+            if (p < packs) write(out, p, v[i], y, c, prob);
+        }
+        for (int i = 0; i < Q; ++i) {
+            const int p = (R + i) * NT + threadIdx.x;
+            if (p < packs) write(out, p, lds[i * NT + threadIdx.x], y, c, prob);
         }
         const int at = packs * PK::N + threadIdx.x;
         if (at < vocab) out[at] = (T)(prob(tail) + (at == y ? c : 0.f));
@@ -557,14 +596,15 @@ struct HeldRow {
 };
 
 // Logits to gradient with one read: a row's coefficient needs the whole row's
-// statistics, so the row stays in registers until they are known.  REST: rows
-// longer than R NT packs; what does not fit is read again.
-// Bound by memory: 4,096 x 131,072 bf16 442 us (4.9 TB/s; reading the row a
-// second time instead of holding it 547), 1,021 x 50,257 f32 85 us.  A row of
-// 256 KB fills a CU's registers, so the exponentials of its two passes (17 us
-// of its 27) overlap only with other CUs' memory.  Loading the next row into
-// the registers that the gradient frees spilled them (882 us) and was left out.
-template <typename T, int NT, int R, bool REST>
+// statistics, so the row stays on the CU until they are known.  REST: rows
+// longer than (R + Q) NT packs; what does not fit is read again, from the
+// Infinity Cache.
+// Bound by memory: 4,096 x 131,072 bf16 415 us (5.2 TB/s; reading all of the
+// row a second time instead of holding it 547), 1,021 x 50,257 f32 85 us.  The
+// exponentials of a row's two passes take two thirds of its time, so another
+// row has to be on the CU beside it.  Loading the next row into the registers
+// that the gradient frees spilled them (882 us).
+template <typename T, int NT, int R, int Q, bool REST>
 __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t stride, int vocab, const void *target,
                                                     int target_bits, ExpScale k, double tau, bool once, dlr_policy p,
                                                     PolicyOut po, T *out, int64_t out_stride) {
@@ -578,10 +618,12 @@ __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t str
         if (out) zero_row<T, NT>(out + t * out_stride, vocab);
         return;
     }
-    constexpr int kHeld = R * NT * Pack<T>::N;
+    constexpr int kHeld = (R + Q) * NT * Pack<T>::N;
+    __shared__ u32x4 stash[Q ? Q * NT : 1];
     const int here = REST ? kHeld : vocab;
     const T *row = logits + t * stride;
-    HeldRow<T, NT, R> held;
+    HeldRow<T, NT, R, Q> held;
+    held.lds = stash;
     held.load(row, here, once);
     const float zy = y < vocab ? (float)row[y] : __builtin_nanf("");
     RowStat own = held.stat(here, k);
@@ -1386,20 +1428,21 @@ hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const 
     });
 }
 
-template <typename T, int NT, int R, bool REST = false>
+template <typename T, int NT, int R, int Q = 0, bool REST = false>
 static hipError_t launch_policy(hipStream_t st, const dlr_logits &x, const dlr_policy &p, const PolicyOut &po,
                                 void *out, int64_t out_stride) {
-    return launch(k_policy_loss<T, NT, R, REST>, x.rows, NT, st, static_cast<const T *>(x.data), x.row_stride,
+    return launch(k_policy_loss<T, NT, R, Q, REST>, x.rows, NT, st, static_cast<const T *>(x.data), x.row_stride,
                   (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature), x.temperature, read_once(x), p, po,
                   static_cast<T *>(out), out_stride);
 }
 
-// The smallest workgroup whose registers hold a row: the more of them on a CU,
-// the more of a row's two passes overlap with other rows' memory (bf16, us, the
-// row held by 512 / 1,024 threads: 4,096 x 65,536 204 / 254, 8,192 x 32,000 186
-// / 189; 8,000 x 1,000 by 128 / 256: 14 / 18).  Rows longer than a CU's
-// registers hold what fits beside the second reading's own (16 packs a thread
-// spill 16-bit types there: 1,024 x 200,000 386 us, with 8 204).
+// The smallest workgroup that holds a row: the more of them on a CU, the more of
+// a row's two passes overlap with other rows' memory (bf16, us, the row held by
+// 512 / 1,024 threads: 4,096 x 65,536 204 / 254, 8,192 x 32,000 186 / 189;
+// 8,000 x 1,000 by 128 / 256: 14 / 18).  Longer rows: two workgroups a CU that
+// hold 136 KB each, in registers and LDS, and read what is left again beat one
+// that holds all in 16 bits, whose passes compute twice as much per byte (4,096
+// x 131,072 415 / 463, 1,024 x 200,000 177 / 192), not in 32 (921 / 900).
 hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, void *workspace, float *loss,
                               float *logprob, float *kl, uint8_t *clipped, void *out, int64_t out_stride) {
     const PolicyOut po{loss, logprob, kl, clipped};
@@ -1417,9 +1460,13 @@ hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_pol
         if (packs <= 512) return launch_policy<T, 128, 4>(st, x, p, po, out, out_stride);
         if (packs <= 1024) return launch_policy<T, 256, 4>(st, x, p, po, out, out_stride);
         if (packs <= 4096) return launch_policy<T, 512, 8>(st, x, p, po, out, out_stride);
+        if constexpr (sizeof(T) == 2) {
+            if (packs <= 17 * 512) return launch_policy<T, 512, 16, 1>(st, x, p, po, out, out_stride);
+            return launch_policy<T, 512, 8, 9, true>(st, x, p, po, out, out_stride);
+        }
         if (packs <= 8192) return launch_policy<T, 512, 16>(st, x, p, po, out, out_stride);
         if (packs <= 16384) return launch_policy<T, 1024, 16>(st, x, p, po, out, out_stride);
-        return launch_policy<T, 1024, sizeof(T) == 4 ? 16 : 8, true>(st, x, p, po, out, out_stride);
+        return launch_policy<T, 1024, 16, 0, true>(st, x, p, po, out, out_stride);
     });
 }
 

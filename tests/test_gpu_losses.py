@@ -828,3 +828,42 @@ def test_preference_with_an_impossible_sequence(L):
     assert out.loss[0] == inf
     out = L.preference_loss(worse, None, off, beta=0.5, label_smoothing=1.0)  # all weight on the other side
     assert out.loss[0] == inf
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("vocab", [8192, 16388, 32776, 65543, 69632, 69647, 131075])
+def test_long_rows_of_many(L, vocab, dtype):
+    # more rows than go by chunks, on both sides of what a workgroup holds of a row
+    rows, tau, lo, hi, klc = 131, 0.8, 0.2, 0.3, 0.05
+    z, z64 = make_logits(rows, vocab, DTYPES[dtype], 1)
+    y = make_target(rows, vocab, ignore=(1,))
+    y[0], y[2], y[3] = vocab - 1, 0, min(vocab - 1, 69632)
+    edit = torch.zeros(4, vocab)
+    edit[2, vocab // 2:] = -math.inf  # nothing left in the second half
+    edit[3, :] = -math.inf            # nothing but the given class
+    edit[3, y[3]] = 0.0
+    z[:4] += edit.to(z.dtype).cuda()
+    pick = torch.tensor([0, 1, 2, 3, 64, 129, 130])
+    z64 = z64[pick]
+    z64[:4] += edit.double()
+    some = y[pick]
+    lp, lse = ref_logprob(z64, some, tau)
+    e = lse_tol(vocab)
+    got_lp, got_lse = L.token_logprob(z, y.cuda(), temperature=tau)
+    close(got_lp[pick], lp, e + U * lp.abs())
+    close(got_lse[pick], lse, e + U * lse.abs())
+    old, ref, adv, w = policy_inputs(rows, 3, torch.full((rows,), -5.0, dtype=torch.float64))
+    old[pick], ref[pick] = (lp + 0.2).float(), (lp - 0.3).float()
+    used = (some >= 0) & (w[pick] != 0)
+    loss, kl, clipped, coef, size = ref_policy(lp, old[pick], ref[pick], adv[pick], w[pick], lo, hi, klc)
+    args = (y.cuda(), old.cuda(), adv.cuda())
+    more = dict(ref_logprob=ref.cuda(), weight=w.cuda(), clip_low=lo, clip_high=hi, kl_coef=klc, temperature=tau)
+    out = L.policy_loss(z, *args, **more)
+    zero = torch.zeros_like(lp)
+    close(out.logprob[pick], torch.where(used, lp, zero), e + U * lp.abs())
+    close(out.loss[pick], torch.where(used, loss, zero), 2 * e * size + 2 * U * loss.abs() + 2 * U * kl)
+    assert torch.equal(out.clipped.cpu()[pick], clipped & used)
+    check_grad(out.grad[pick], z64, some, torch.where(used, coef, zero),
+               w[pick].double() * (2 * e * size) + 2 * U * coef.abs(), tau, extra=e)
+    same = L.policy_loss(z, *args, **more, out=z)
+    assert same.grad is z and torch.equal(z, out.grad) and torch.equal(same.loss, out.loss)
