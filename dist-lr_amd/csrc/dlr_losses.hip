@@ -686,10 +686,11 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     for (int i = 0; i < 2; ++i) {
         first[i] = p.offsets[pair + i * P];
         last[i] = p.offsets[pair + i * P + 1];
-        if (first[i] < 0 || last[i] < first[i] || last[i] > T) {  // no range of the tokens: not read, not written
-            bad = true;
-            first[i] = last[i] = 0;
-        }
+        // No range of the tokens: what lies within them gets the pair's NaN, so
+        // that every token's gradient is written.
+        if (first[i] < 0 || last[i] < first[i] || last[i] > T) bad = true;
+        first[i] = first[i] < 0 ? 0 : first[i] > T ? T : first[i];
+        last[i] = last[i] < first[i] ? first[i] : last[i] > T ? T : last[i];
     }
     const int64_t b = q ? first[1] : first[0], e = q ? last[1] : last[0];
     auto mask4 = [&](int64_t i) { return p.mask ? *reinterpret_cast<const u32_any *>(p.mask + i) : 0x01010101u; };
@@ -750,7 +751,7 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     }
     if (!o.grad) return;
     // d loss / d u = sigma(u) - (1 - eps)
-    const double slope = w == 0.0 ? 0.0 : w * (eps / (1.0 + exp(-u)) - (1.0 - eps) / (1.0 + exp(u)));
+    const double slope = w == 0.0 && !bad ? 0.0 : w * (eps / (1.0 + exp(-u)) - (1.0 - eps) / (1.0 + exp(u)));
     const float g = (float)(q ? -slope * scale[1] : slope * scale[0]);
 #pragma unroll 4
     for (int64_t v = at; v < packs; v += H) {

@@ -128,9 +128,9 @@ int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_pol
  *   u        = reward_p - reward_{pairs+p} - margin
  *   loss[p]  = -(1 - label_smoothing) log sigma(u) - label_smoothing log sigma(-u)
  * The objective is sum_p weight[p] * loss[p]; grad is its gradient with
- * respect to logprob: tokens without mask and tokens of no sequence get 0
- * (their log-probabilities are not read).  Offsets that are no ranges of the
- * tokens give NaN for their pair. */
+ * respect to logprob: tokens without mask and tokens of no sequence get 0,
+ * whatever their log-probabilities hold.  Offsets that are no ranges of the
+ * tokens give NaN for their pair and its tokens. */
 typedef struct dlr_preference {
     const float *logprob;       /* tokens                                     */
     const float *ref_logprob;   /* tokens; NULL: 0                            */

@@ -867,3 +867,20 @@ def test_long_rows_of_many(L, vocab, dtype):
                w[pick].double() * (2 * e * size) + 2 * U * coef.abs(), tau, extra=e)
     same = L.policy_loss(z, *args, **more, out=z)
     assert same.grad is z and torch.equal(z, out.grad) and torch.equal(same.loss, out.loss)
+
+
+def test_preference_bad_offsets_write_every_gradient(L):
+    import ctypes
+    inf = float("inf")
+    for bad, want in (([-1, 2, 4, 6, 8], "nnggnngg00"), ([0, 2, 4, 6, 11], "ggnnggnnnn"),
+                      ([0, 1 << 62, 4, 6, 8], "nnnnnnnn??"), ([3, 4, 5, 6, 20], "000gngnnnn")):
+        lp, off = torch.randn(10).cuda(), torch.tensor(bad).cuda()
+        out = torch.full((3, 2), inf).cuda()
+        grad = torch.full((10,), inf).cuda()
+        p = L._Preference(lp.data_ptr(), None, None, off.data_ptr(), None, 2, 10, 0.1, 0.0, 0.0, 0, 0)
+        L._check(L.lib.dlr_preference_loss(0, L._stream(0), ctypes.byref(p), *(o.data_ptr() for o in out),
+                                           grad.data_ptr()))
+        g = grad.cpu()
+        for token, kind in enumerate(want):
+            v = float(g[token])
+            assert {"n": math.isnan(v), "g": 0 < abs(v) < 0.1, "0": v == 0, "?": v != inf}[kind], (bad, token, v)
