@@ -58,10 +58,12 @@ bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
     return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
 }
 
-constexpr int64_t kMaxRows = INT64_C(0x7fffffff);  // one workgroup per row
+constexpr int64_t kMaxRows = INT64_C(0x7fffffff);
+constexpr int64_t kMaxPairs = (INT64_C(1) << 22) - 1;  // one launch of at most 1,024 threads each
 constexpr int64_t kMaxVocab = INT64_C(1) << 30;
 constexpr int64_t kMaxDim = INT64_C(1) << 20;
-constexpr int64_t kMaxLogits = INT64_C(1) << 44;  // a head call's: its tiles are one launch
+constexpr int64_t kMaxClasses = INT64_C(1) << 28;  // a head call's
+constexpr int64_t kMaxLogits = INT64_C(1) << 44;
 
 const char *check_target(const void *target, int32_t bits, double temperature) {
     if (!target) return "target is NULL";
@@ -192,7 +194,7 @@ int dlr_preference_loss(int device, void *stream, const dlr_preference *p, float
                         float *rejected_reward, float *grad) {
     const char *call = "dlr_preference_loss";
     if (!p) return refuse(DLR_E_ARG, call, "the descriptor is NULL");
-    if (p->pairs < 0 || p->pairs > kMaxRows / 2) return refuse(DLR_E_ARG, call, "pairs must be 0 .. 2^30 - 1");
+    if (p->pairs < 0 || p->pairs > kMaxPairs) return refuse(DLR_E_ARG, call, "pairs must be 0 .. 2^22 - 1");
     if (p->tokens < 0 || p->tokens > (INT64_C(1) << 40)) return refuse(DLR_E_ARG, call, "tokens must be 0 .. 2^40");
     if (!(p->beta > 0.0) || !std::isfinite(p->beta)) return refuse(DLR_E_ARG, call, "beta must be positive and finite");
     if (!(p->label_smoothing >= 0.0 && p->label_smoothing <= 1.0))
@@ -219,7 +221,7 @@ int dlr_preference_loss(int device, void *stream, const dlr_preference *p, float
 }
 
 int64_t dlr_head_logprob_workspace(int64_t rows, int64_t vocab, int64_t dim) {
-    if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || dim < 1 || dim > kMaxDim ||
+    if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxClasses || dim < 1 || dim > kMaxDim ||
         rows * vocab > kMaxLogits)
         return refuse(DLR_E_ARG, "dlr_head_logprob_workspace", "rows, vocab or dim is out of range");
     return dlr::head_workspace(rows, vocab, dim);
@@ -230,7 +232,7 @@ int dlr_head_logprob(int device, void *stream, const dlr_head *h, void *workspac
     const char *call = "dlr_head_logprob";
     if (!h) return refuse(DLR_E_ARG, call, "the descriptor is NULL");
     if (h->rows < 0 || h->rows > kMaxRows) return refuse(DLR_E_ARG, call, "rows must be 0 .. 2^31 - 1");
-    if (h->vocab < 1 || h->vocab > kMaxVocab) return refuse(DLR_E_ARG, call, "vocab must be 1 .. 2^30");
+    if (h->vocab < 1 || h->vocab > kMaxClasses) return refuse(DLR_E_ARG, call, "vocab must be 1 .. 2^28");
     if (h->dim < 1 || h->dim > kMaxDim) return refuse(DLR_E_ARG, call, "dim must be 1 .. 2^20");
     if (h->rows * h->vocab > kMaxLogits) return refuse(DLR_E_ARG, call, "rows * vocab must be at most 2^44");
     if (h->dtype != DLR_DTYPE_BF16 && h->dtype != DLR_DTYPE_F16)

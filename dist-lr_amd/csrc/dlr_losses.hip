@@ -1338,6 +1338,36 @@ static hipError_t by_dtype(int dtype, F f) {
 
 constexpr int64_t kCus = 256;
 
+// A launch has fewer than 2^32 threads: more rows than this go by several
+// launches of about as many (never by a few: row_parts' workspace is the whole
+// call's).
+constexpr int64_t kLaunchRows = INT64_C(1) << 21;
+
+// f(rows at .. of `x`, at), slice by slice; at least one row.
+template <typename X, typename F>
+static hipError_t by_rows(const X &x, int64_t most, F f) {
+    const int64_t slices = (x.rows + most - 1) / most, each = (x.rows + slices - 1) / slices;
+    hipError_t e = hipSuccess;
+    for (int64_t at = 0; at < x.rows && e == hipSuccess; at += each) {
+        X part = x;
+        part.target = static_cast<const char *>(x.target) + at * (x.target_bits / 8);
+        part.rows = x.rows - at < each ? x.rows - at : each;
+        e = f(part, at);
+    }
+    return e;
+}
+
+// The same with the logits' type as f's first argument.
+template <typename F>
+static hipError_t by_logits(const dlr_logits &whole, F f) {
+    return by_rows(whole, kLaunchRows, [&](dlr_logits &x, int64_t at) {
+        return by_dtype(x.dtype, [&](auto e) {
+            x.data = static_cast<const decltype(e) *>(x.data) + at * x.row_stride;
+            return f(e, x, at);
+        });
+    });
+}
+
 // Logits of more bytes than the 256 MB Infinity Cache cannot be there when the
 // call begins, nor will a second read find them: they are read past it.
 constexpr int64_t kOnceBytes = INT64_C(1) << 28;
@@ -1382,9 +1412,10 @@ static hipError_t launch_logprob(hipStream_t st, const dlr_logits &x, float *log
                   x.target, x.target_bits, exp_scale(x.temperature), x.temperature, read_once(x), logprob, lse);
 }
 
-hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, void *workspace, float *logprob, float *lse) {
-    return by_dtype(x.dtype, [&](auto e) {
+hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &all, void *workspace, float *logprobs, float *lses) {
+    return by_logits(all, [&](auto e, const dlr_logits &x, int64_t at) {
         using T = decltype(e);
+        float *logprob = logprobs + at, *lse = lses + at;
         const RowParts w = row_parts(x.rows, x.vocab, Pack<T>::N, workspace);
         if (w.chunks > 1) {
             const hipError_t r = launch_parts<T>(st, x, nullptr, w);
@@ -1409,10 +1440,12 @@ static hipError_t launch_grad(hipStream_t st, const dlr_logits &x, const float *
 // As above; rows of 2,048 to 16,384 packs gain from fewer of them in flight
 // at once (8,192 x 32,000 bf16 191 -> 174 us with 1,024 threads a row), longer
 // ones lose (4,096 x 131,072 f32 810 -> 864).
-hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad,
-                                     void *out, int64_t out_stride) {
-    return by_dtype(x.dtype, [&](auto e) {
+hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &all, const float *lses, const float *grads,
+                                     void *outs, int64_t out_stride) {
+    return by_logits(all, [&](auto e, const dlr_logits &x, int64_t at) {
         using T = decltype(e);
+        const float *lse = lses + at, *grad = grads + at;
+        T *out = static_cast<T *>(outs) + at * out_stride;
         const int64_t packs = x.vocab / Pack<T>::N;
         // Few long rows by chunks of 1,024 packs and more, four workgroups a CU
         // in all (1 x 131,072 bf16: 2.9 us, 10.6 by one workgroup); not over
@@ -1444,11 +1477,18 @@ static hipError_t launch_policy(hipStream_t st, const dlr_logits &x, const dlr_p
 // hold 136 KB each, in registers and LDS, and read what is left again beat one
 // that holds all in 16 bits, whose passes compute twice as much per byte (4,096
 // x 131,072 415 / 463, 1,024 x 200,000 177 / 192), not in 32 (921 / 900).
-hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, void *workspace, float *loss,
-                              float *logprob, float *kl, uint8_t *clipped, void *out, int64_t out_stride) {
-    const PolicyOut po{loss, logprob, kl, clipped};
-    return by_dtype(x.dtype, [&](auto e) {
+hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &all, const dlr_policy &policy, void *workspace,
+                              float *loss, float *logprob, float *kl, uint8_t *clipped, void *outs,
+                              int64_t out_stride) {
+    return by_logits(all, [&](auto e, const dlr_logits &x, int64_t at) {
         using T = decltype(e);
+        dlr_policy p = policy;
+        p.old_logprob += at;
+        p.advantage += at;
+        if (p.ref_logprob) p.ref_logprob += at;
+        if (p.weight) p.weight += at;
+        const PolicyOut po{loss + at, logprob + at, kl + at, clipped + at};
+        T *out = outs ? static_cast<T *>(outs) + at * out_stride : nullptr;
         const RowParts w = row_parts(x.rows, x.vocab, Pack<T>::N, workspace);
         if (w.chunks > 1) {
             const hipError_t r = launch_parts<T>(st, x, p.weight, w);
@@ -1604,7 +1644,7 @@ constexpr int64_t kFewTiles = 128;
 // 4096: 131,072 classes 180 us against 190, 65,536 classes 118 against 105).
 static int64_t few_rows_tile(int64_t vocab) { return vocab >= 2 * kCus * 192 ? 256 : 64; }
 
-int64_t head_workspace(int64_t rows, int64_t vocab, int64_t dim) {
+static int64_t head_slice_workspace(int64_t rows, int64_t vocab, int64_t dim) {
     int64_t tiles = tiles_of(vocab, few_rows_tile(vocab));
     if (rows > 16) {
         const HeadPlan plan = head_plan(rows, vocab, dim);
@@ -1613,6 +1653,21 @@ int64_t head_workspace(int64_t rows, int64_t vocab, int64_t dim) {
     }
     const int64_t plain = tiles_of(vocab, kTileV);  // unaligned rows
     return head_part(rows) + rows * (tiles > plain ? tiles : plain) * (int64_t)sizeof(float2);
+}
+
+// The rows of one run of launches, whose workgroups of 256 threads for 64 x 64
+// logits stay below 2^32 threads; each slice uses the workspace again.
+static int64_t head_rows(int64_t vocab) {
+    const int64_t most = (INT64_C(1) << 35) / vocab;
+    return most < kLaunchRows ? most : kLaunchRows;
+}
+
+int64_t head_workspace(int64_t rows, int64_t vocab, int64_t dim) {
+    const int64_t slices = (rows + head_rows(vocab) - 1) / head_rows(vocab);
+    if (slices <= 1) return head_slice_workspace(rows, vocab, dim);
+    const int64_t each = (rows + slices - 1) / slices, last = rows - (rows - 1) / each * each;
+    const int64_t a = head_slice_workspace(each, vocab, dim), b = head_slice_workspace(last, vocab, dim);
+    return a > b ? a : b;
 }
 
 template <typename T>
@@ -1644,7 +1699,7 @@ static hipError_t launch_head_tiles(hipStream_t st, const dlr_head &h, const Hea
     return e != hipSuccess || plan.classes == h.vocab ? e : by(plan.rest, plan.classes, h.vocab);
 }
 
-hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
+static hipError_t launch_head_slice(hipStream_t st, const dlr_head &h, void *workspace, float *logprob, float *lse) {
     const HeadSpace w = head_space(workspace, h.rows);
     const bool picks = head_by_dma(h) && head_picks(h);
     const HeadPick pick{picks ? w.row : nullptr, w.count};
@@ -1659,6 +1714,13 @@ hipError_t launch_head_logprob(hipStream_t st, const dlr_head &h, void *workspac
     return h.rows < 16 ? launch(k_head_join<1>, h.rows, 256, st, h, pick, tiles, w.part, w.zy, logprob, lse)
                        : launch(k_head_join<16>, (h.rows + 15) / 16, 256, st, h, pick, tiles, w.part, w.zy, logprob,
                                 lse);
+}
+
+hipError_t launch_head_logprob(hipStream_t st, const dlr_head &all, void *workspace, float *logprob, float *lse) {
+    return by_rows(all, head_rows(all.vocab), [&](dlr_head &h, int64_t at) {
+        h.hidden = static_cast<const uint16_t *>(h.hidden) + at * h.hidden_stride;
+        return launch_head_slice(st, h, workspace, logprob + at, lse + at);
+    });
 }
 
 }  // namespace dlr

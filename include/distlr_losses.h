@@ -36,6 +36,8 @@
  *   - Errors: DLR_E_ARG for arguments that do not fit (message through
  *     dlr_losses_last_error()), nothing is enqueued then; DLR_E_HIP if the launch
  *     fails.  rows = 0 is a valid call that does nothing.
+ *   - Up to 2^31 - 1 rows; from 2^21 (dlr_head_logprob: 2^35 logits) on a
+ *     call is several launches, which a failing one ends.
  *   - A library of its own: it needs neither the engine nor RCCL, and it
  *     shares its caller's HIP runtime, whose streams and tensors it takes.  It
  *     is linked to the name "libamdhip64.so", under which torch loads its
@@ -137,8 +139,8 @@ typedef struct dlr_preference {
     const uint8_t *mask;        /* tokens, 0 = does not count; NULL: all do   */
     const int64_t *offsets;     /* 2 * pairs + 1, ascending                   */
     const float *weight;        /* pairs; NULL: 1                             */
-    int64_t pairs;
-    int64_t tokens;
+    int64_t pairs;              /* 0 .. 2^22 - 1                              */
+    int64_t tokens;             /* 0 .. 2^40                                  */
     double beta;                /* > 0                                        */
     double label_smoothing;     /* in [0, 1]                                  */
     double margin;
@@ -157,7 +159,8 @@ typedef struct dlr_head {
     const void *hidden;         /* rows x dim                                 */
     const void *head;           /* vocab x dim: one row of weights per class  */
     const void *target;
-    int64_t rows, vocab, dim;   /* dim 1 .. 2^20, rows * vocab <= 2^44        */
+    int64_t rows, vocab, dim;   /* vocab 1 .. 2^28, dim 1 .. 2^20,            */
+                                /* rows * vocab <= 2^44                       */
     int64_t hidden_stride;      /* elements between rows                      */
     int64_t head_stride;
     int32_t dtype;

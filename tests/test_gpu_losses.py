@@ -884,3 +884,60 @@ def test_preference_bad_offsets_write_every_gradient(L):
         for token, kind in enumerate(want):
             v = float(g[token])
             assert {"n": math.isnan(v), "g": 0 < abs(v) < 0.1, "0": v == 0, "?": v != inf}[kind], (bad, token, v)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_rows_than_one_launch(L, dtype):
+    # from 2^21 rows on a call is several launches; a row's results depend on the row alone
+    rows, vocab, many = 1000, 9, (1 << 21) + 5
+    times = many // rows + 1
+    z, z64 = make_logits(rows, vocab, DTYPES[dtype])
+    y = make_target(rows, vocab, ignore=(1,))
+    lp, lse = L.token_logprob(z, y.cuda())
+    want = ref_logprob(z64, y, 1.0)[0]
+    close(lp, want, lse_tol(vocab) + U * want.abs())
+    g = torch.randn(rows, generator=gen(5)).cuda()
+    old, ref, adv, w = (t.cuda() for t in policy_inputs(rows, 3, want))
+
+    def over(t):
+        return t.repeat(times, *[1] * (t.dim() - 1))[:many]
+
+    def all_of(z, y, lse, g, old, ref, adv, w):
+        yield from L.token_logprob(z, y)
+        yield L.token_logprob_grad(z, y, lse, g)
+        yield from L.policy_loss(z, y, old, adv, ref_logprob=ref, weight=w, kl_coef=0.1)
+
+    few = (z, y.cuda(), lse, g, old, ref, adv, w)
+    for got, want in zip(all_of(*(over(t) for t in few)), all_of(*few)):
+        assert torch.equal(got, over(want))
+    yy = over(y.cuda())
+    zz = over(z).contiguous()
+    want = L.token_logprob_grad(z, y.cuda(), lse, g)
+    assert torch.equal(L.token_logprob_grad(zz, yy, over(lse), over(g), out=zz), over(want))
+    if dtype == "bf16":
+        hidden = torch.randn(rows, 16, generator=gen(8)).bfloat16().cuda()
+        head = torch.randn(vocab, 16, generator=gen(9)).bfloat16().cuda()
+        e = 2 * (lse_tol(vocab) + U * 36 + 32 * U * float((hidden.double().abs() @ head.double().abs().t()).max()))
+        for got, want in zip(L.head_logprob(over(hidden), head, yy), L.head_logprob(hidden, head, y.cuda())):
+            close(got, over(want).cpu().double(), (e + 2 * U * over(want).abs()).cpu().double())
+
+
+def test_head_of_more_logits_than_one_launch(L):
+    # from 2^35 logits on a call is several runs of launches over one workspace
+    rows, vocab, dim, scale = 8292, (1 << 22) + 77, 8, 4.0
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    x = torch.randint(-2, 3, (rows, dim), generator=g, device="cuda").bfloat16()
+    w = torch.randint(-2, 3, (vocab, dim), generator=g, device="cuda").bfloat16()
+    y = make_target(rows, vocab)
+    y[torch.rand(rows, generator=gen(4)) < 0.5] = -1
+    pick = torch.tensor([0, 1, 2, 4145, 4146, 4147, 8290, 8291])
+    y[pick] = make_target(8, vocab, seed=9)
+    lp, lse = L.head_logprob(x, w, y.cuda(), temperature=scale)
+    z = torch.mm(x[pick.cuda()].double(), w.double().t()).cpu()  # whole numbers: exact
+    want_lp, want_lse = ref_logprob(z, y[pick], scale)
+    e = lse_tol(vocab) + U * 3 * 12
+    close(lse[pick], want_lse, e + U * want_lse.abs())
+    close(lp[pick], want_lp, e + U * want_lp.abs())
+    out = (y < 0).cuda()
+    assert (lp[out] == 0).all() and (lse[out] == 0).all() and (lse[~out] > 0).all() and (lp[~out] < 0).all()

@@ -244,3 +244,24 @@ def test_tensors_off_the_gpu_are_refused():
         with pytest.raises(dlr.DLRError) as e:
             call()
         assert e.value.code == dlr.E_ARG
+
+
+def test_calls_beyond_one_launch():
+    # more pairs or classes than a launch has threads for are refused, more rows go by several launches
+    p = L._Preference(A, None, None, B, None, 1 << 22, 10, 0.1, 0.0, 0.0, 0, 0)
+    rc, msg = code(L.lib.dlr_preference_loss(0, None, C.byref(p), D, D, D, E))
+    assert rc == dlr.E_ARG and "pairs" in msg
+    size = L.lib.dlr_head_logprob_workspace
+    assert code(size(1, (1 << 28) + 1, 64))[0] == dlr.E_ARG and size(1, 1 << 28, 64) > 0
+    h = L._Head(A, A, B, 1, (1 << 28) + 1, 64, 64, 64, L.DTYPE_BF16, 64, 1.0)
+    rc, msg = code(L.lib.dlr_head_logprob(0, None, C.byref(h), D, 1 << 40, E, E))
+    assert rc == dlr.E_ARG and "vocab" in msg
+    # scratch memory is a slice's, whatever the call's rows (a tile's 8 bytes a row, at most one for 64 classes)
+    for vocab in (7, 4096, 131072, 1 << 24):
+        most = min(1 << 21, (1 << 35) // vocab)
+        for rows in (most, most + 1, 2 * most + 1, 5 * most, min((1 << 31) - 1, (1 << 44) // vocab)):
+            need = size(rows, vocab, 512)
+            assert need <= most * 8 * (vocab // 64 + 3) + 512
+            slices = -(-rows // most)
+            each = -(-rows // slices)
+            assert need >= size(each, vocab, 512) and need >= size(rows - (rows - 1) // each * each, vocab, 512)
