@@ -115,21 +115,6 @@ bool floats(std::initializer_list<const void *> ps) {
     return true;
 }
 
-int token_logprob(const char *call, int device, void *stream, const dlr_logits *x, void *workspace,
-                  int64_t workspace_bytes, void *logprob, bool wide, float *lse) {
-    if (const char *why = check_logits(x)) return refuse(DLR_E_ARG, call, why);
-    if (x->rows == 0) return DLR_OK;
-    if (!logprob || !lse) return refuse(DLR_E_ARG, call, "logprob or lse is NULL");
-    if (!aligned(logprob, wide ? 8 : 4) || !aligned(lse, 4))
-        return refuse(DLR_E_ARG, call, "logprob or lse is not aligned");
-    if (const char *why = check_workspace(workspace, workspace_bytes, dlr::logits_workspace(x->rows, x->vocab, x->dtype)))
-        return refuse(DLR_E_ARG, call, why);
-    DeviceScope d(device);
-    if (d.error() != hipSuccess) return fail_hip(call, d.error());
-    const hipError_t e = dlr::launch_token_logprob(static_cast<hipStream_t>(stream), *x, workspace, logprob, wide, lse);
-    return e == hipSuccess ? DLR_OK : fail_hip(call, e);
-}
-
 }  // namespace
 
 extern "C" {
@@ -149,12 +134,17 @@ int64_t dlr_logits_workspace(int64_t rows, int64_t vocab, int dtype) {
 
 int dlr_token_logprob(int device, void *stream, const dlr_logits *x, void *workspace, int64_t workspace_bytes,
                       float *logprob, float *lse) {
-    return token_logprob("dlr_token_logprob", device, stream, x, workspace, workspace_bytes, logprob, false, lse);
-}
-
-int dlr_token_logprob64(int device, void *stream, const dlr_logits *x, void *workspace, int64_t workspace_bytes,
-                        double *logprob, float *lse) {
-    return token_logprob("dlr_token_logprob64", device, stream, x, workspace, workspace_bytes, logprob, true, lse);
+    const char *call = "dlr_token_logprob";
+    if (const char *why = check_logits(x)) return refuse(DLR_E_ARG, call, why);
+    if (x->rows == 0) return DLR_OK;
+    if (!logprob || !lse) return refuse(DLR_E_ARG, call, "logprob or lse is NULL");
+    if (!floats({logprob, lse})) return refuse(DLR_E_ARG, call, "logprob or lse is not aligned");
+    if (const char *why = check_workspace(workspace, workspace_bytes, dlr::logits_workspace(x->rows, x->vocab, x->dtype)))
+        return refuse(DLR_E_ARG, call, why);
+    DeviceScope d(device);
+    if (d.error() != hipSuccess) return fail_hip(call, d.error());
+    const hipError_t e = dlr::launch_token_logprob(static_cast<hipStream_t>(stream), *x, workspace, logprob, lse);
+    return e == hipSuccess ? DLR_OK : fail_hip(call, e);
 }
 
 int dlr_token_logprob_grad(int device, void *stream, const dlr_logits *x, const float *lse, const float *grad,
@@ -211,22 +201,16 @@ int dlr_preference_loss(int device, void *stream, const dlr_preference *p, float
         return refuse(DLR_E_ARG, call, "label_smoothing must lie in [0, 1]");
     if (!std::isfinite(p->margin)) return refuse(DLR_E_ARG, call, "margin must be finite");
     if (p->average != 0 && p->average != 1) return refuse(DLR_E_ARG, call, "average must be 0 or 1");
-    for (int32_t bits : {p->logprob_bits, p->ref_bits})
-        if (bits != 0 && bits != 32 && bits != 64)
-            return refuse(DLR_E_ARG, call, "logprob_bits and ref_bits must be 0, 32 or 64");
-    const int64_t bytes = p->logprob_bits == 64 ? 8 : 4, ref_bytes = p->ref_bits == 64 ? 8 : 4;
     if (p->pairs == 0 && (p->tokens == 0 || !grad)) return DLR_OK;
     if (p->pairs && (!p->offsets || !loss || !chosen_reward || !rejected_reward))
         return refuse(DLR_E_ARG, call, "offsets or an output is NULL");
     if (p->pairs && p->tokens && !p->logprob) return refuse(DLR_E_ARG, call, "logprob is NULL");
-    if (!aligned(p->logprob, bytes) || !aligned(p->ref_logprob, ref_bytes) ||
-        !floats({p->weight, loss, chosen_reward, rejected_reward, grad}))
+    if (!floats({p->logprob, p->ref_logprob, p->weight, loss, chosen_reward, rejected_reward, grad}))
         return refuse(DLR_E_ARG, call, "a float array is not aligned");
     if (!aligned(p->offsets, 8)) return refuse(DLR_E_ARG, call, "offsets is not aligned");
     if (grad && p->tokens) {
         const int64_t b = p->tokens * 4;
-        if (overlap(grad, b, p->logprob, p->tokens * bytes) ||
-            (p->ref_logprob && overlap(grad, b, p->ref_logprob, p->tokens * ref_bytes)))
+        if (overlap(grad, b, p->logprob, b) || (p->ref_logprob && overlap(grad, b, p->ref_logprob, b)))
             return refuse(DLR_E_ARG, call, "grad overlaps an input");
     }
     DeviceScope d(device);

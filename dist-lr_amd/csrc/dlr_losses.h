@@ -13,9 +13,7 @@ namespace dlr {
 
 // Bytes of scratch memory of launch_token_logprob and launch_policy_loss.
 int64_t logits_workspace(int64_t rows, int64_t vocab, int32_t dtype);
-// logprob: doubles if `wide`, else floats.
-hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, void *workspace, void *logprob, bool wide,
-                                float *lse);
+hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &x, void *workspace, float *logprob, float *lse);
 hipError_t launch_token_logprob_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad,
                                      void *out, int64_t out_stride);
 hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &x, const dlr_policy &p, void *workspace, float *loss,

@@ -245,32 +245,19 @@ __device__ inline double target_logprob(float zy, float m, double ln_s, double t
 
 // ----------------------------------------------------- token log-probabilities
 
-// Log-probabilities in 32 or 64 bits.  Rounded to 32 they are exact enough but
-// for sums that nearly cancel against another model's: a sequence's reward is
-// off by 1e-7 of its log-probabilities, all there is of one that is near 0.
-struct LogprobOut {
-    void *p;
-    bool wide;
-    __device__ void set(int64_t t, double v) const {
-        if (wide) static_cast<double *>(p)[t] = v;
-        else static_cast<float *>(p)[t] = (float)v;
-    }
-    LogprobOut from(int64_t t) const { return {static_cast<char *>(p) + t * (wide ? 8 : 4), wide}; }
-};
-
 // One row a workgroup, one read.  Bound by memory: 4,096 x 131,072 bf16, a
 // quarter of the rows out, 141 us, 5.7 TB/s of what is read (the exponentials
 // alone would take 55 us); short and few rows by the row's ends.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t stride, int vocab, const void *target,
-                                                      int target_bits, ExpScale k, double tau, bool once,
-                                                      LogprobOut logprob, float *lse) {
+                                                      int target_bits, ExpScale k, double tau, bool once, float *logprob,
+                                                      float *lse) {
     __shared__ BlockLds<NT> lds;
     const int64_t t = blockIdx.x;
     const int64_t y = load_target(target, target_bits, t);
     if (y < 0) {  // ignored: the row is not read
         if (threadIdx.x == 0) {
-            logprob.set(t, 0.0);
+            logprob[t] = 0.f;
             lse[t] = 0.f;
         }
         return;
@@ -281,7 +268,7 @@ __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t s
     if (threadIdx.x == 0) {
         const double ln = log(a.s);
         lse[t] = (float)(a.m / tau + ln);
-        logprob.set(t, target_logprob(zy, a.m, ln, tau));
+        logprob[t] = (float)target_logprob(zy, a.m, ln, tau);
     }
 }
 
@@ -333,21 +320,18 @@ __device__ inline BlockStat join_parts(const RowParts &w, int64_t t, ExpScale k)
 }
 
 __global__ __launch_bounds__(64) void k_token_finish(const void *target, int target_bits, int vocab, ExpScale k,
-                                                     double tau, RowParts w, LogprobOut logprob, float *lse) {
+                                                     double tau, RowParts w, float *logprob, float *lse) {
     const int64_t t = blockIdx.x;
     const int64_t y = load_target(target, target_bits, t);
     if (y < 0) {
-        if (threadIdx.x == 0) {
-            logprob.set(t, 0.0);
-            lse[t] = 0.f;
-        }
+        if (threadIdx.x == 0) logprob[t] = lse[t] = 0.f;
         return;
     }
     const BlockStat a = join_parts(w, t, k);
     if (threadIdx.x == 0) {
         const double ln = log(a.s);
         lse[t] = (float)(a.m / tau + ln);
-        logprob.set(t, target_logprob(y < vocab ? w.zy[t] : __builtin_nanf(""), a.m, ln, tau));
+        logprob[t] = (float)target_logprob(y < vocab ? w.zy[t] : __builtin_nanf(""), a.m, ln, tau);
     }
 }
 
@@ -668,22 +652,7 @@ struct PairOut {
 __device__ inline double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
-typedef double f64x4 __attribute__((ext_vector_type(4)));
-typedef f64x4 f64x4_any __attribute__((aligned(8)));
-
 typedef uint32_t u32_any __attribute__((aligned(1)));
-
-// Log-probabilities of type V: token i's, and those of tokens i .. i + 3 as
-// they lie (converted where they are used: doubles at once cost registers).
-template <typename V>
-__device__ inline double token1(const void *x, int64_t i) {
-    return static_cast<const V *>(x)[i];
-}
-template <typename V>
-__device__ inline auto token4(const void *x, int64_t i) {
-    if constexpr (sizeof(V) == 8) return (f64x4) * reinterpret_cast<const f64x4_any *>(static_cast<const double *>(x) + i);
-    else return (f32x4) * reinterpret_cast<const f32x4_any *>(static_cast<const float *>(x) + i);
-}
 
 // One pair a workgroup, half of it for each sequence: the sums of log ratios
 // in 64 bits (they nearly cancel), the logistic loss of their difference, and
@@ -694,8 +663,7 @@ __device__ inline auto token4(const void *x, int64_t i) {
 // behind its mask), two pairs 4.  One workgroup a pair also where the
 // sequences are very long (1 x 400,000 tokens 69 us): the logits of such a
 // pair take a thousand times as long.
-// L, R: the types of logprob and ref_logprob.
-template <typename L, typename R, int NT>
+template <int NT>
 __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOut o) {
     constexpr int H = NT / 2, W = NT / 64;
     __shared__ double sums[W];
@@ -733,9 +701,9 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     for (int64_t v = at; v < packs; v += H) {
         const int64_t i = b + 4 * v;
         const uint32_t m = mask4(i);
-        const auto l = token4<L>(p.logprob, i);
-        decltype(token4<R>(nullptr, 0)) r = {};
-        if (p.ref_logprob) r = token4<R>(p.ref_logprob, i);
+        const f32x4 l = *reinterpret_cast<const f32x4_any *>(p.logprob + i);
+        f32x4 r = {};
+        if (p.ref_logprob) r = *reinterpret_cast<const f32x4_any *>(p.ref_logprob + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const bool on = (m >> (8 * j)) & 0xff;
@@ -745,7 +713,7 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     }
     const bool tail_on = tail < e && (!p.mask || p.mask[tail]);
     if (tail_on) {
-        sum += token1<L>(p.logprob, tail) - (p.ref_logprob ? token1<R>(p.ref_logprob, tail) : 0.0);
+        sum += (double)p.logprob[tail] - (p.ref_logprob ? (double)p.ref_logprob[tail] : 0.0);
         count += 1;
     }
 #pragma unroll
@@ -1439,17 +1407,15 @@ static hipError_t launch_parts(hipStream_t st, const dlr_logits &x, const float 
 // (1 x 32,000: 4.9 us with 512, 12.8 with 64; 4,096 x 131,072: 189 against
 // 195).
 template <typename T, int NT>
-static hipError_t launch_logprob(hipStream_t st, const dlr_logits &x, const LogprobOut &logprob, float *lse) {
+static hipError_t launch_logprob(hipStream_t st, const dlr_logits &x, float *logprob, float *lse) {
     return launch(k_token_logprob<T, NT>, x.rows, NT, st, static_cast<const T *>(x.data), x.row_stride, (int)x.vocab,
                   x.target, x.target_bits, exp_scale(x.temperature), x.temperature, read_once(x), logprob, lse);
 }
 
-hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &all, void *workspace, void *logprobs, bool wide,
-                                float *lses) {
+hipError_t launch_token_logprob(hipStream_t st, const dlr_logits &all, void *workspace, float *logprobs, float *lses) {
     return by_logits(all, [&](auto e, const dlr_logits &x, int64_t at) {
         using T = decltype(e);
-        const LogprobOut logprob = LogprobOut{logprobs, wide}.from(at);
-        float *lse = lses + at;
+        float *logprob = logprobs + at, *lse = lses + at;
         const RowParts w = row_parts(x.rows, x.vocab, Pack<T>::N, workspace);
         if (w.chunks > 1) {
             const hipError_t r = launch_parts<T>(st, x, nullptr, w);
@@ -1545,24 +1511,17 @@ hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &all, const dlr_p
     });
 }
 
-template <typename L, typename R>
-static hipError_t launch_preference(hipStream_t st, const dlr_preference &p, const PairOut &o) {
+hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float *loss, float *chosen,
+                                  float *rejected, float *grad) {
     const int64_t blocks = p.pairs ? p.pairs : 1;
+    const PairOut o{loss, chosen, rejected, grad};
     // A large workgroup for long sequences, where there are CUs for it (us by
     // 256 / 512 / 1,024 threads: 16 pairs of 1,000 tokens 5.7 / 4.7 / 5.3, 1,024
     // of 1,465 11 / 12 / 19, 64 of 23,400 - / 30 / 23).
     const int64_t each = p.tokens / blocks;
-    if (each > 8192) return launch(k_preference_loss<L, R, 1024>, blocks, 1024, st, p, o);
-    if (each > 512 && blocks <= 2 * kCus) return launch(k_preference_loss<L, R, 512>, blocks, 512, st, p, o);
-    return launch(k_preference_loss<L, R, 256>, blocks, 256, st, p, o);
-}
-
-hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float *loss, float *chosen,
-                                  float *rejected, float *grad) {
-    const PairOut o{loss, chosen, rejected, grad};
-    if (p.logprob_bits == 64)
-        return p.ref_bits == 64 ? launch_preference<double, double>(st, p, o) : launch_preference<double, float>(st, p, o);
-    return p.ref_bits == 64 ? launch_preference<float, double>(st, p, o) : launch_preference<float, float>(st, p, o);
+    if (each > 8192) return launch(k_preference_loss<1024>, blocks, 1024, st, p, o);
+    if (each > 512 && blocks <= 2 * kCus) return launch(k_preference_loss<512>, blocks, 512, st, p, o);
+    return launch(k_preference_loss<256>, blocks, 256, st, p, o);
 }
 
 // Whether the rows can go through the DMA kernels: 16-byte chunks of rows that

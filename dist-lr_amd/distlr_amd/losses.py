@@ -38,7 +38,6 @@ SYMBOLS = {
     "dlr_losses_runtime": (C.c_char_p,),
     "dlr_logits_workspace": (i64, i64, i64, C.c_int),
     "dlr_token_logprob": (C.c_int, C.c_int, P, P, P, i64, P, P),
-    "dlr_token_logprob64": (C.c_int, C.c_int, P, P, P, i64, P, P),
     "dlr_token_logprob_grad": (C.c_int, C.c_int, P, P, P, P, P, i64),
     "dlr_policy_loss": (C.c_int, C.c_int, P, P, P, P, i64, P, P, P, P, P, i64),
     "dlr_preference_loss": (C.c_int, C.c_int, P, P, P, P, P, P),
@@ -78,7 +77,7 @@ class _Preference(C.Structure):
     _fields_ = [("logprob", C.c_void_p), ("ref_logprob", C.c_void_p), ("mask", C.c_void_p), ("offsets", C.c_void_p),
                 ("weight", C.c_void_p), ("pairs", C.c_int64), ("tokens", C.c_int64), ("beta", C.c_double),
                 ("label_smoothing", C.c_double), ("margin", C.c_double), ("average", C.c_int32),
-                ("reserved", C.c_int32), ("logprob_bits", C.c_int32), ("ref_bits", C.c_int32)]
+                ("reserved", C.c_int32)]
 
 
 class _Head(C.Structure):
@@ -138,7 +137,6 @@ def _vector(name: str, t, gpu: int, dtypes, length: int) -> torch.Tensor:
 
 
 _F32 = (torch.float32,)
-_F32_64 = (torch.float32, torch.float64)
 _INTS = (torch.int64, torch.int32)
 _BOOL = (torch.bool,)
 
@@ -189,28 +187,17 @@ def _scratch(x: _Logits, like: torch.Tensor):
 _stream = torch._C._cuda_getCurrentRawStream
 
 
-def token_logprob(logits: torch.Tensor, target: torch.Tensor, *, temperature: float = 1.0,
-                  dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(logprob, lse) per row: logprob = logits[t, target[t]] / temperature -
-    lse, lse = log sum exp(logits[t] / temperature).  A negative target marks
-    a row that takes no part: 0, not read (dlr_token_logprob).
-
-    dtype is logprob's: float64 for sums that nearly cancel against another
-    model's, as preference_loss's rewards (dlr_token_logprob64).  lse is
-    float32."""
+def token_logprob(logits: torch.Tensor, target: torch.Tensor, *,
+                  temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(logprob, lse), float32 per row: logprob = logits[t, target[t]] /
+    temperature - lse, lse = log sum exp(logits[t] / temperature).  A
+    negative target marks a row that takes no part: 0, not read
+    (dlr_token_logprob)."""
     gpu, target, x = _logits(logits, target, temperature)
+    out, at = _rows(2, x.rows, logits)
     need, scratch = _scratch(x, logits)
-    if dtype is torch.float32:
-        out, at = _rows(2, x.rows, logits)
-        _check(lib.dlr_token_logprob(gpu, _stream(gpu), C.byref(x), _ptr(scratch), need, at, at + 4 * x.rows))
-        return out
-    if dtype is not torch.float64:
-        _refuse(f"dtype must be torch.float32 or torch.float64 (it is {dtype})")
-    logprob = torch.empty(x.rows, dtype=dtype, device=logits.device)
-    lse = torch.empty(x.rows, dtype=torch.float32, device=logits.device)
-    _check(lib.dlr_token_logprob64(gpu, _stream(gpu), C.byref(x), _ptr(scratch), need, logprob.data_ptr(),
-                                   lse.data_ptr()))
-    return logprob, lse
+    _check(lib.dlr_token_logprob(gpu, _stream(gpu), C.byref(x), _ptr(scratch), need, at, at + 4 * x.rows))
+    return out
 
 
 def token_logprob_grad(logits: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor, *,
@@ -276,15 +263,14 @@ def preference_loss(logprob: torch.Tensor, ref_logprob: Optional[torch.Tensor], 
     reward = beta * sum(logprob - ref_logprob) over the tokens with mask
     (average: per counted token); loss = -(1 - label_smoothing) log sigma(u) -
     label_smoothing log sigma(-u), u = chosen_reward - rejected_reward -
-    margin.  weight (P) defaults to 1.  logprob and ref_logprob are float32
-    or float64, each; the results and the gradient are float32."""
+    margin.  weight (P) defaults to 1."""
     gpu = _gpu("logprob", logprob)
     if logprob.dim() != 1:
         _refuse(f"logprob must have 1 dimension (it has {logprob.dim()})")
     tokens = logprob.shape[0]
-    logprob = _vector("logprob", logprob, gpu, _F32_64, tokens)
+    logprob = _vector("logprob", logprob, gpu, _F32, tokens)
     if ref_logprob is not None:
-        ref_logprob = _vector("ref_logprob", ref_logprob, gpu, _F32_64, tokens)
+        ref_logprob = _vector("ref_logprob", ref_logprob, gpu, _F32, tokens)
     _gpu("offsets", offsets)
     if offsets.dim() != 1 or offsets.shape[0] % 2 != 1:
         _refuse("offsets must have 2 P + 1 entries")
@@ -295,10 +281,9 @@ def preference_loss(logprob: torch.Tensor, ref_logprob: Optional[torch.Tensor], 
     if weight is not None:
         weight = _vector("weight", weight, gpu, _F32, pairs)
     p = _Preference(logprob.data_ptr(), _ptr(ref_logprob), _ptr(mask), offsets.data_ptr(), _ptr(weight), pairs, tokens,
-                    beta, label_smoothing, margin, 1 if average else 0, 0, 8 * logprob.element_size(),
-                    32 if ref_logprob is None else 8 * ref_logprob.element_size())
+                    beta, label_smoothing, margin, 1 if average else 0, 0)
     (loss, chosen, rejected), at = _rows(3, pairs, logprob)
-    dl = torch.empty_like(logprob, dtype=torch.float32) if grad else None
+    dl = torch.empty_like(logprob) if grad else None
     _check(lib.dlr_preference_loss(gpu, _stream(gpu), C.byref(p), at, at + 4 * pairs, at + 8 * pairs, _ptr(dl)))
     return PreferenceLoss(loss, chosen, rejected, dl)
 

@@ -88,10 +88,6 @@ int64_t dlr_logits_workspace(int64_t rows, int64_t vocab, int dtype);
  * - lse[t], y = target[t].  Each logit is read once. */
 int dlr_token_logprob(int device, void *stream, const dlr_logits *x, void *workspace, int64_t workspace_bytes,
                       float *logprob, float *lse);
-/* The same with log-probabilities in 64 bits, for sums of them that nearly
- * cancel against another model's (dlr_preference_loss's rewards). */
-int dlr_token_logprob64(int device, void *stream, const dlr_logits *x, void *workspace, int64_t workspace_bytes,
-                        double *logprob, float *lse);
 
 /* The gradient of sum_t grad[t] * logprob[t] with respect to the logits (the
  * softmax residual): grad_logits[t][j] = grad[t] / temperature * (1[j = y] -
@@ -138,8 +134,8 @@ int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_pol
  * whatever their log-probabilities hold.  Offsets that are no ranges of the
  * tokens give NaN for their pair and its tokens. */
 typedef struct dlr_preference {
-    const void *logprob;        /* tokens, of logprob_bits                    */
-    const void *ref_logprob;    /* tokens, of ref_bits; NULL: 0               */
+    const float *logprob;       /* tokens                                     */
+    const float *ref_logprob;   /* tokens; NULL: 0                            */
     const uint8_t *mask;        /* tokens, 0 = does not count; NULL: all do   */
     const int64_t *offsets;     /* 2 * pairs + 1, ascending                   */
     const float *weight;        /* pairs; NULL: 1                             */
@@ -149,9 +145,7 @@ typedef struct dlr_preference {
     double label_smoothing;     /* in [0, 1]                                  */
     double margin;
     int32_t average;            /* 1: rewards per counted token               */
-    int32_t reserved;           /* 0                                          */
-    int32_t logprob_bits;       /* 0 or 32: float, 64: double                 */
-    int32_t ref_bits;
+    int32_t reserved;
 } dlr_preference;
 /* loss, chosen_reward, rejected_reward: pairs each.  grad: tokens, or NULL. */
 int dlr_preference_loss(int device, void *stream, const dlr_preference *p, float *loss, float *chosen_reward,

@@ -941,67 +941,3 @@ def test_head_of_more_logits_than_one_launch(L):
     close(lp[pick], want_lp, e + U * want_lp.abs())
     out = (y < 0).cuda()
     assert (lp[out] == 0).all() and (lse[out] == 0).all() and (lse[~out] > 0).all() and (lp[~out] < 0).all()
-
-
-@pytest.mark.parametrize("rows,vocab", [(1, 7), (9, 5003), (3, 140003), (140, 1001)])
-def test_logprob_in_64_bits(L, rows, vocab):
-    for dtype in DTYPES.values():
-        z, z64 = make_logits(rows, vocab, dtype, 1)
-        y = make_target(rows, vocab, ignore=(1,))
-        lp, lse = L.token_logprob(z, y.cuda(), temperature=0.7)
-        wide, same = L.token_logprob(z, y.cuda(), temperature=0.7, dtype=torch.float64)
-        assert wide.dtype == torch.float64 and torch.equal(wide.float(), lp) and torch.equal(same, lse)
-        want, _ = ref_logprob(z64, y, 0.7)
-        close(wide, want, torch.full((rows,), lse_tol(vocab)).double() + 1e-13)  # nothing of its own size is rounded
-
-
-@pytest.mark.parametrize("lengths", list(LENGTHS))
-@pytest.mark.parametrize("wide", [(True, True), (True, False), (False, True)])
-def test_preference_in_64_bits(L, lengths, wide):
-    n = LENGTHS[lengths]
-    offsets = [0]
-    for k in n:
-        offsets.append(offsets[-1] + k)
-    T, P = offsets[-1], len(n) // 2
-    g = gen(len(n) + T)
-    lp = -torch.rand(T, generator=g).double() * 6
-    ref = lp + 1e-6 * torch.randn(T, generator=g).double()  # two models that hardly differ
-    lp, ref = (t if w else t.float() for t, w in zip((lp, ref), wide))
-    mask = torch.rand(T, generator=g) < 0.7
-    off = torch.tensor(offsets).cuda()
-    store = torch.full((T + 1,), float("nan"), dtype=lp.dtype).cuda()
-    store[1:] = lp.cuda()
-    for m in (None, mask):
-        want = ref_preference(lp, ref, offsets, 0.3, mask=m)
-        got = L.preference_loss(store[1:], ref.cuda(), off, beta=0.3, mask=None if m is None else m.cuda())
-        assert all(t.dtype == torch.float32 for t in got)
-        for a, b in zip(got, want):
-            # sums of up to 9,001 differences of at most 7e-6, exact to 2^-53 of the 6 they come from
-            close(a, b, 1.01 * U * b.abs() + 1e-11)
-
-
-def test_a_reward_near_zero_keeps_its_digits(L):
-    # all there is of these rewards is what a 32-bit log-probability would round away
-    z, _ = make_logits(64, 1000, torch.float32)
-    lp, _ = L.token_logprob(z, make_target(64, 1000).cuda(), dtype=torch.float64)
-    ref = lp.float()
-    out = L.preference_loss(lp, ref, torch.tensor([0, 32, 64]).cuda(), beta=1.0)
-    gap = (lp - ref.double()).cpu()
-    for got, want in ((out.chosen_reward, gap[:32].sum()), (out.rejected_reward, gap[32:].sum())):
-        assert 0 < abs(want) < 1e-4 and abs(float(got) - want) <= U * abs(want) + 32 * 1e-4 * 2.0 ** -52
-
-
-def test_types_of_log_probabilities(L, dlr):
-    z, _ = make_logits(4, 100, torch.float32)
-    y = make_target(4, 100).cuda()
-    off = torch.tensor([0, 2, 4]).cuda()
-    for bad in (torch.bfloat16, torch.float16, torch.int64, None):
-        with pytest.raises(dlr.DLRError):
-            L.token_logprob(z, y, dtype=bad)
-    for bad in (torch.bfloat16, torch.float16):
-        with pytest.raises(dlr.DLRError):
-            L.preference_loss(torch.zeros(4, dtype=bad).cuda(), None, off, beta=1.0)
-        with pytest.raises(dlr.DLRError):
-            L.preference_loss(torch.zeros(4).cuda(), torch.zeros(4, dtype=bad).cuda(), off, beta=1.0)
-    lp, lse = L.token_logprob(z[:0], y[:0], dtype=torch.float64)
-    assert lp.shape == (0,) and lse.shape == (0,) and lp.dtype == torch.float64

@@ -265,26 +265,3 @@ def test_calls_beyond_one_launch():
             slices = -(-rows // most)
             each = -(-rows // slices)
             assert need >= size(each, vocab, 512) and need >= size(rows - (rows - 1) // each * each, vocab, 512)
-
-
-@pytest.mark.parametrize("kw,word", [
-    (dict(logprob_bits=16), "bits"), (dict(ref_bits=8), "bits"), (dict(logprob=A + 4, logprob_bits=64), "aligned"),
-    (dict(ref_logprob=B + 4, ref_bits=64), "aligned")])
-def test_bad_types_of_log_probabilities(kw, word):
-    v = dict(logprob=A, ref_logprob=None, mask=None, offsets=B, weight=None, pairs=2, tokens=10, beta=0.1,
-             label_smoothing=0.0, margin=0.0, average=0, reserved=0)
-    v.update(kw)
-    p = L._Preference(**v)
-    rc, msg = code(L.lib.dlr_preference_loss(0, None, C.byref(p), D, D, D, E))
-    assert rc == dlr.E_ARG and word in msg
-    # doubles reach twice as far
-    p = L._Preference(A, None, None, B, None, 2, 10, 0.1, 0.0, 0.0, 0, 0, 64, 0)
-    rc, msg = code(L.lib.dlr_preference_loss(0, None, C.byref(p), D, D, D, A + 76))
-    assert rc == dlr.E_ARG and "overlap" in msg
-
-
-def test_bad_64_bit_log_probabilities():
-    x = L._Logits(A, B, 4, 100, 100, L.DTYPE_F32, 64, 1.0)
-    for logprob, lse, word in ((None, E, "NULL"), (D, None, "NULL"), (D + 4, E, "aligned"), (D, E + 2, "aligned")):
-        rc, msg = code(L.lib.dlr_token_logprob64(0, None, C.byref(x), None, 0, logprob, lse))
-        assert rc == dlr.E_ARG and word in msg and "dlr_token_logprob64" in msg
