@@ -1258,14 +1258,15 @@ __global__ __launch_bounds__(256) void k_head_waves(dlr_head h, int64_t v_first,
 }
 
 // The tiles' statistics, joined: RT tokens a workgroup (their statistics lie
-// side by side), 256 / RT threads each.  The maximum first, then the scaled
-// sums in 64 bits (as join_block); a thread keeps its first 16 tiles.
-template <int RT>
-__global__ __launch_bounds__(256) void k_head_join(dlr_head h, HeadPick pick, int64_t tiles, const float2 *part,
-                                                   const float *zy, float *logprob, float *lse) {
-    constexpr int G = 256 / RT, K = 16;
-    __shared__ float lm[4][RT];
-    __shared__ double ls[4][RT];
+// side by side), NT / RT threads each.  The maximum first, then the scaled
+// sums in 64 bits (as join_block); a thread keeps its first 16 tiles.  Bound by
+// its trips to memory, 5 to 7 us up to 1,000 tokens.
+template <int RT, int NT>
+__global__ __launch_bounds__(NT) void k_head_join(dlr_head h, HeadPick pick, int64_t tiles, const float2 *part,
+                                                  const float *zy, float *logprob, float *lse) {
+    constexpr int G = NT / RT, K = 16, W = NT / 64;
+    __shared__ float lm[W][RT];
+    __shared__ double ls[W][RT];
     const int tok = threadIdx.x % RT, first = threadIdx.x / RT, wave = threadIdx.x >> 6;
     const int64_t t = (int64_t)blockIdx.x * RT + tok, used = pick.row ? *pick.count : h.rows;
     const bool in = t < used;
@@ -1284,16 +1285,20 @@ __global__ __launch_bounds__(256) void k_head_join(dlr_head h, HeadPick pick, in
     float m = NEG_INF;
 #pragma unroll
     for (int i = 0; i < K; ++i) m = fmaxf(m, q[i].x);
+#pragma unroll 4
     for (int64_t n = first + K * G; n < tiles; n += G) m = fmaxf(m, p[n * h.rows].x);
 #pragma unroll
     for (int o = RT; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
     if ((threadIdx.x & 63) < RT) lm[wave][tok] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(lm[0][tok], lm[1][tok]), fmaxf(lm[2][tok], lm[3][tok]));
+    m = lm[0][tok];
+#pragma unroll
+    for (int w = 1; w < W; ++w) m = fmaxf(m, lm[w][tok]);
     const float r = m == NEG_INF ? 0.f : m;
     double s = 0.0;
 #pragma unroll
     for (int i = 0; i < K; ++i) s += (double)q[i].y * (double)exp2_scaled(q[i].x - r, k);
+#pragma unroll 4
     for (int64_t n = first + K * G; n < tiles; n += G) {
         const float2 v = p[n * h.rows];
         s += (double)v.y * (double)exp2_scaled(v.x - r, k);
@@ -1303,7 +1308,9 @@ __global__ __launch_bounds__(256) void k_head_join(dlr_head h, HeadPick pick, in
     if ((threadIdx.x & 63) < RT) ls[wave][tok] = s;
     __syncthreads();
     if (first || !in) return;
-    s = (ls[0][tok] + ls[1][tok]) + (ls[2][tok] + ls[3][tok]);
+    s = ls[0][tok];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += ls[w][tok];
     const double tau = h.temperature, ln = log(s);
     lse[row] = y < 0 ? 0.f : (float)(m / tau + ln);
     logprob[row] = y < 0 ? 0.f : (float)target_logprob(z, m, ln, tau);
@@ -1711,9 +1718,13 @@ static hipError_t launch_head_slice(hipStream_t st, const dlr_head &h, void *wor
         e = h.dtype == DLR_DTYPE_BF16 ? launch_head_tiles<__bf16>(st, h, pick, w, tiles)
                                       : launch_head_tiles<_Float16>(st, h, pick, w, tiles);
     if (e != hipSuccess) return e;
-    return h.rows < 16 ? launch(k_head_join<1>, h.rows, 256, st, h, pick, tiles, w.part, w.zy, logprob, lse)
-                       : launch(k_head_join<16>, (h.rows + 15) / 16, 256, st, h, pick, tiles, w.part, w.zy, logprob,
-                                lse);
+    if (h.rows < 16) return launch(k_head_join<1, 256>, h.rows, 256, st, h, pick, tiles, w.part, w.zy, logprob, lse);
+    // 256 threads a token while every CU has a workgroup, else 64 (24 tokens of
+    // 1,757 tiles 6.5 us, 12.2; 343 of 891 6.5, 9.7; 4,096 of 512 22.6, 7.9; 16
+    // threads 42, 27, 11.4).
+    if (h.rows <= 4 * kCus)
+        return launch(k_head_join<4, 1024>, (h.rows + 3) / 4, 1024, st, h, pick, tiles, w.part, w.zy, logprob, lse);
+    return launch(k_head_join<16, 1024>, (h.rows + 15) / 16, 1024, st, h, pick, tiles, w.part, w.zy, logprob, lse);
 }
 
 hipError_t launch_head_logprob(hipStream_t st, const dlr_head &all, void *workspace, float *logprob, float *lse) {
