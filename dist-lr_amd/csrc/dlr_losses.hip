@@ -965,6 +965,14 @@ __global__ __launch_bounds__(WV *WT * 64) void k_head_dma(dlr_head h, int64_t v_
     // one; a wave without an L-th load repeats the last load (every wave then
     // has L of them in flight per stage).
     const char *src[L];  // of the stage to be filled next
+    // The whole stages in a circle, then the short one: class tiles begin a stage
+    // apart, or, where rows lie a power of two apart, all workgroups would read
+    // from few memory channels at a time (128 x 4096 x 65536 149 us from the same
+    // stage, 115; 256 x 4096 x 65536 174, 145).  Not up to 16 tokens, whose two
+    // workgroups a CU drift apart by themselves (1 x 4096 x 131072 178, 183).
+    constexpr bool kCircle = TT > 16;
+    const int start = kCircle && full > 0 ? (int)(vt % full) : 0;
+    int at_stage = start, left = full;
     const int chunk = (lane & 7) ^ (lane >> 3);
     auto load_no = [&](int q) {
         const int n = wave * L + q;
@@ -979,21 +987,31 @@ __global__ __launch_bounds__(WV *WT * 64) void k_head_dma(dlr_head h, int64_t v_
         int64_t at = first + r < last ? first + r : last;
         if (x) at = token(at);
         src[q] = static_cast<const char *>(x ? h.hidden : h.head) + at * (x ? h.hidden_stride : h.head_stride) * 2 +
-                 chunk * 16;
+                 chunk * 16 + start * 128;
     }
+    auto step_on = [&]() {  // bytes to the next stage
+        if constexpr (!kCircle) return (int64_t)128;
+        int next = at_stage + 1 < full ? at_stage + 1 : 0;
+        if (--left == 0) next = full;
+        const int64_t by = (int64_t)(next - at_stage) * 128;
+        at_stage = next;
+        return by;
+    };
     auto fill = [&](int buf) {
+        const int64_t by = step_on();
 #pragma unroll
         for (int q = 0; q < L; ++q) {
             lds_dma16(src[q], sm[buf] + load_no(q) * 1024);
-            src[q] += 128;
+            src[q] += by;
         }
     };
     auto fill_last = [&](int step, int buf) {  // a stage that may be short (dim is a multiple of 8): zeros behind it
-        const bool in = step * 64 + chunk * 8 < dim;
+        const bool in = step < full || step * 64 + chunk * 8 < dim;
+        const int64_t by = step_on();
 #pragma unroll
         for (int q = 0; q < L; ++q) {
             lds_dma16(in ? src[q] : (const char *)&kZero16, sm[buf] + load_no(q) * 1024);
-            src[q] += 128;
+            src[q] += by;
         }
     };
     struct Frag {
