@@ -119,6 +119,10 @@ def _gpu(name: str, t) -> int:
 def _matrix(name: str, t: torch.Tensor, gpu: int) -> None:
     if _gpu(name, t) != gpu:
         _refuse(f"{name} is on GPU {t.get_device()}, not on GPU {gpu}")
+    _rows_of(name, t)
+
+
+def _rows_of(name: str, t: torch.Tensor) -> None:
     if t.dim() != 2:
         _refuse(f"{name} must have 2 dimensions (it has {t.dim()})")
     if t.stride(1) != 1 and t.shape[1] > 1:
@@ -127,13 +131,14 @@ def _matrix(name: str, t: torch.Tensor, gpu: int) -> None:
 
 def _vector(name: str, t, gpu: int, dtypes, length: int) -> torch.Tensor:
     """A 1-D tensor of one of `dtypes`; a strided one is copied."""
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == gpu and t.dtype in dtypes
+            and t.shape == (length,)):
+        return t if t.is_contiguous() else t.contiguous()
     if _gpu(name, t) != gpu:
         _refuse(f"{name} is on GPU {t.get_device()}, not on GPU {gpu}")
     if t.dtype not in dtypes:
         _refuse(f"{name} must be {' or '.join(str(d) for d in dtypes)} (it is {t.dtype})")
-    if t.dim() != 1 or t.shape[0] != length:
-        _refuse(f"{name} must have shape ({length},) (it has {tuple(t.shape)})")
-    return t if t.is_contiguous() else t.contiguous()
+    _refuse(f"{name} must have shape ({length},) (it has {tuple(t.shape)})")
 
 
 _F32 = (torch.float32,)
@@ -147,7 +152,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _logits(logits: torch.Tensor, target: torch.Tensor, temperature: float):
     gpu = _gpu("logits", logits)
-    _matrix("logits", logits, gpu)
+    _rows_of("logits", logits)
     if logits.dtype not in _DTYPES:
         _refuse(f"logits must be float32, bfloat16 or float16 (they are {logits.dtype})")
     rows, vocab = logits.shape
@@ -167,9 +172,8 @@ def _grad_like(logits: torch.Tensor, out: Optional[torch.Tensor], gpu: int) -> t
     return out
 
 
-def _rows(count: int, length: int, like: torch.Tensor):
-    """`count` float32 vectors side by side in one allocation, and its address."""
-    out = torch.empty((count, length), dtype=torch.float32, device=like.device)
+def _rows(out: torch.Tensor):
+    """Vectors side by side in one allocation, and its address."""
     return out.unbind(0), out.data_ptr()
 
 
@@ -194,7 +198,7 @@ def token_logprob(logits: torch.Tensor, target: torch.Tensor, *,
     negative target marks a row that takes no part: 0, not read
     (dlr_token_logprob)."""
     gpu, target, x = _logits(logits, target, temperature)
-    out, at = _rows(2, x.rows, logits)
+    out, at = _rows(torch.empty((2, x.rows), dtype=torch.float32, device=logits.device))
     need, scratch = _scratch(x, logits)
     _check(lib.dlr_token_logprob(gpu, _stream(gpu), C.byref(x), _ptr(scratch), need, at, at + 4 * x.rows))
     return out
@@ -242,7 +246,7 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logprob: torch.T
     dz = _grad_like(logits, out, gpu) if grad else None
     p = _Policy(old_logprob.data_ptr(), _ptr(ref_logprob), advantage.data_ptr(), _ptr(weight), clip_low, clip_high,
                 kl_coef)
-    (loss, logprob, kl), at = _rows(3, rows, logits)
+    (loss, logprob, kl), at = _rows(old_logprob.new_empty((3, rows)))  # float32: 0.3 us less than torch.empty
     clipped = torch.empty(rows, dtype=torch.bool, device=logits.device)
     need, scratch = _scratch(x, logits)
     _check(lib.dlr_policy_loss(gpu, _stream(gpu), C.byref(x), C.byref(p), _ptr(scratch), need, at, at + 4 * rows,
@@ -282,7 +286,7 @@ def preference_loss(logprob: torch.Tensor, ref_logprob: Optional[torch.Tensor], 
         weight = _vector("weight", weight, gpu, _F32, pairs)
     p = _Preference(logprob.data_ptr(), _ptr(ref_logprob), _ptr(mask), offsets.data_ptr(), _ptr(weight), pairs, tokens,
                     beta, label_smoothing, margin, 1 if average else 0, 0)
-    (loss, chosen, rejected), at = _rows(3, pairs, logprob)
+    (loss, chosen, rejected), at = _rows(logprob.new_empty((3, pairs)))
     dl = torch.empty_like(logprob) if grad else None
     _check(lib.dlr_preference_loss(gpu, _stream(gpu), C.byref(p), at, at + 4 * pairs, at + 8 * pairs, _ptr(dl)))
     return PreferenceLoss(loss, chosen, rejected, dl)
@@ -294,7 +298,7 @@ def head_logprob(hidden: torch.Tensor, head: torch.Tensor, target: torch.Tensor,
     which are never written out: scoring by a model that is not trained.
     bfloat16 or float16, sums in 32 bits (dlr_head_logprob)."""
     gpu = _gpu("hidden", hidden)
-    _matrix("hidden", hidden, gpu)
+    _rows_of("hidden", hidden)
     _matrix("head", head, gpu)
     if hidden.dtype not in (torch.bfloat16, torch.float16) or head.dtype != hidden.dtype:
         _refuse(f"hidden and head must both be bfloat16 or float16 (they are {hidden.dtype} and {head.dtype})")
@@ -306,6 +310,6 @@ def head_logprob(hidden: torch.Tensor, head: torch.Tensor, target: torch.Tensor,
               head.stride(0), _DTYPES[hidden.dtype], _TARGET_BITS[target.dtype], temperature)
     need = _check(lib.dlr_head_logprob_workspace(rows, head.shape[0], dim))
     workspace = torch.empty(need, dtype=torch.uint8, device=hidden.device)
-    out, at = _rows(2, rows, hidden)
+    out, at = _rows(torch.empty((2, rows), dtype=torch.float32, device=hidden.device))
     _check(lib.dlr_head_logprob(gpu, _stream(gpu), C.byref(h), workspace.data_ptr(), need, at, at + 4 * rows))
     return out
