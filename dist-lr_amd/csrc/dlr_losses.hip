@@ -33,22 +33,25 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// k = hi + lo of the row statistics.  One float for k is off by up to 2^-25,
-// always to the same side: lse would be off by that share of the mean |d|
-// (1e-7 for logits of a trained model, as much as float32's own rounding).
+// k = hi + lo of the row statistics and of the gradients.  One float for k is
+// off by up to 2^-23 (rounded down), always to the same side: lse would be off
+// by that share of the mean |d| (1e-7 for logits of a trained model, as much as
+// float32's own rounding), a gradient's probabilities by that share of their
+// own |d| (1.7e-6 in the mean of 50,257 at temperature 0.7).
 // The other roundings are of either sign and average out over a row; so does
 // v_exp_f32's (mean -3e-9, at most 8e-8, measured over [-24, 0]).
 // hi is k rounded down and lo > 0, so that d = -inf gives -inf twice.
 struct ExpScale {
     float hi, lo;
 };
-__host__ __device__ inline ExpScale exp_scale(double temperature) {
-    const double k = 1.44269504088896340736 / temperature;
+__host__ __device__ inline ExpScale two_floats(double k) {  // k > 0
     float hi = (float)k;
-    if ((double)hi > k) hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, hi) - 1u);  // k > 0: one step down
+    if ((double)hi > k) hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, hi) - 1u);  // one step down
     const float lo = (float)(k - (double)hi);
     return {hi, lo > 0.f ? lo : 1e-30f};
 }
+constexpr double kLog2e = 1.44269504088896340736;
+__host__ __device__ inline ExpScale exp_scale(double temperature) { return two_floats(kLog2e / temperature); }
 __device__ inline float exp2_scaled(float d, ExpScale k) { return exp2_hw(__builtin_fmaf(d, k.hi, d * k.lo)); }
 
 // 16 bytes of a row: N elements.
@@ -389,8 +392,8 @@ constexpr float kLseExact = 128.f;
 // 131,072 bf16 379 us (5.7 TB/s), 2,048 x 50,257 f16 with odd rows 71 us (5.1).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int64_t stride, int vocab,
-                                                           const void *target, int target_bits, double tau, bool once,
-                                                           const float *lse, const float *grad, T *out,
+                                                           const void *target, int target_bits, ExpScale k, double tau,
+                                                           bool once, const float *lse, const float *grad, T *out,
                                                            int64_t out_stride, int chunks, int span) {
     const int64_t t = blockIdx.x / chunks;
     const int begin = (int)(blockIdx.x % chunks) * span, here = vocab - begin < span ? vocab - begin : span;
@@ -406,16 +409,23 @@ __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int6
     const float l = lse[t];
     if (fabsf(l) > kLseExact) {
         __shared__ BlockLds<NT> lds;
-        const ExpScale k = exp_scale(tau);
         const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k, false), k, lds);
         const float neg = (float)(-c / a.s), m = a.m;
         residual_row<T, NT, 4>(row + begin, o, here, y - begin, c,
-                               [=](float z) { return neg * exp2_hw((z - m) * k.hi); }, once);
+                               [=](float z) { return neg * exp2_scaled(z - m, k); }, once);
         return;
     }
-    const float it = (float)(1.0 / tau);
-    residual_row<T, NT, 4>(row + begin, o, here, y - begin, c,
-                           [=](float z) { return -c * exp2_hw(__builtin_fmaf(z, it, -l) * 1.44269504f); }, once);
+    // z / tau - l, rounded once, times log2(e); what the first floats of 1 / tau
+    // and log2(e) leave out goes in before the second rounding
+    const ExpScale it = two_floats(1.0 / tau), e = two_floats(kLog2e);
+    const float it_lo = it.lo * e.hi;
+    residual_row<T, NT, 4>(
+        row + begin, o, here, y - begin, c,
+        [=](float z) {
+            const float x = __builtin_fmaf(z, it.hi, -l);
+            return -c * exp2_hw(__builtin_fmaf(x, e.hi, __builtin_fmaf(x, e.lo, z * it_lo)));
+        },
+        once);
 }
 
 // ---------------------------------------------------------------- policy loss
@@ -490,7 +500,7 @@ __global__ __launch_bounds__(NT) void k_policy_finish(const T *logits, int64_t s
     __syncthreads();
     const float c = coef, neg = (float)(-c / a.s), m = a.m;
     residual_row<T, NT, 4>(logits + t * stride + begin, o, here, y - begin, c,
-                           [=](float z) { return neg * exp2_hw((z - m) * k.hi); }, false);
+                           [=](float z) { return neg * exp2_scaled(z - m, k); }, false);
 }
 
 // A row held by its workgroup: R packs a thread in registers, Q in LDS, pack i
@@ -636,7 +646,7 @@ __global__ __launch_bounds__(NT) void k_policy_loss(const T *logits, int64_t str
     if (!out) return;
     __syncthreads();
     const float c = coef, neg = (float)(-c / a.s), m = a.m;
-    auto prob = [=](float z) { return neg * exp2_hw((z - m) * k.hi); };
+    auto prob = [=](float z) { return neg * exp2_scaled(z - m, k); };
     T *o = out + t * out_stride;
     held.residual(o, here, y, c, prob);
     if constexpr (REST) residual_row<T, NT, 4>(row + kHeld, o + kHeld, vocab - kHeld, y - kHeld, c, prob, once);
@@ -1458,8 +1468,8 @@ template <typename T, int NT>
 static hipError_t launch_grad(hipStream_t st, const dlr_logits &x, const float *lse, const float *grad, void *out,
                               int64_t out_stride, int chunks = 1, int span = 1 << 30) {
     return launch(k_token_logprob_grad<T, NT>, x.rows * chunks, NT, st, static_cast<const T *>(x.data), x.row_stride,
-                  (int)x.vocab, x.target, x.target_bits, x.temperature, read_once(x), lse, grad,
-                  static_cast<T *>(out), out_stride, chunks, span);
+                  (int)x.vocab, x.target, x.target_bits, exp_scale(x.temperature), x.temperature, read_once(x), lse,
+                  grad, static_cast<T *>(out), out_stride, chunks, span);
 }
 
 // As above; rows of 2,048 to 16,384 packs gain from fewer of them in flight
