@@ -664,6 +664,16 @@ __device__ inline double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-f
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 
+// Whether offsets[from .. to] descend between two neighbours that this thread
+// looks at.
+template <int NT>
+__device__ inline bool descend(const int64_t *offsets, int64_t from, int64_t to) {
+    bool falls = false;
+#pragma unroll 4
+    for (int64_t i = from + threadIdx.x; i < to; i += NT) falls |= offsets[i + 1] < offsets[i];
+    return falls;
+}
+
 // One pair a workgroup, half of it for each sequence: the sums of log ratios
 // in 64 bits (they nearly cancel), the logistic loss of their difference, and
 // the pair's one slope written over its tokens.  4 tokens a thread and step,
@@ -673,21 +683,28 @@ typedef uint32_t u32_any __attribute__((aligned(1)));
 // behind its mask), two pairs 4.  One workgroup a pair also where the
 // sequences are very long (1 x 400,000 tokens 69 us): the logits of such a
 // pair take a thousand times as long.
+//
+// Offsets that descend anywhere make sequences overlap, and which workgroup
+// would write a shared token's gradient last is nobody's to say: then every pair
+// and token is NaN.  `look`: each workgroup looks through the offsets for itself;
+// else k_preference_order does, behind this launch.
 template <int NT>
-__global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOut o) {
+__global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOut o, bool look) {
     constexpr int H = NT / 2, W = NT / 64;
     __shared__ double sums[W];
     __shared__ int64_t counts[W];
     const int64_t P = p.pairs, T = p.tokens;
-    if (o.grad) {  // tokens of no sequence: before the first, behind the last
-        int64_t b = P ? p.offsets[0] : T, e = P ? p.offsets[2 * P] : T;
-        b = b < 0 ? 0 : b > T ? T : b;
-        e = e < b ? b : e > T ? T : e;
-        const int64_t first = (int64_t)blockIdx.x * NT + threadIdx.x, all = (int64_t)gridDim.x * NT;
-        for (int64_t i = first; i < b; i += all) o.grad[i] = 0.f;
-        for (int64_t i = e + first; i < T; i += all) o.grad[i] = 0.f;
+    // tokens [b, e) of the gradient, by all workgroups
+    auto fill = [&](int64_t b, int64_t e, float v) {
+        for (int64_t i = b + (int64_t)blockIdx.x * NT + threadIdx.x; i < e; i += (int64_t)gridDim.x * NT) o.grad[i] = v;
+    };
+    if (!P) {
+        if (o.grad) fill(0, T, 0.f);
+        return;
     }
-    if (!P) return;
+    const int64_t from = p.offsets[0], to = p.offsets[2 * P];
+    bool falls = false;
+    if (look) falls = descend<NT>(p.offsets, 0, 2 * P);
     const int64_t pair = blockIdx.x;
     const int q = threadIdx.x / H, at = threadIdx.x % H;
     int64_t first[2], last[2];
@@ -735,7 +752,10 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
         sums[threadIdx.x >> 6] = sum;
         counts[threadIdx.x >> 6] = count;
     }
-    __syncthreads();
+    if (look)
+        falls = __syncthreads_or(falls);
+    else
+        __syncthreads();
     double reward[2], scale[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -751,7 +771,7 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     }
     const double eps = p.label_smoothing;
     double u = reward[0] - reward[1] - p.margin;
-    if (bad) u = reward[0] = reward[1] = __builtin_nan("");
+    if (bad || falls) u = reward[0] = reward[1] = __builtin_nan("");
     const double w = p.weight ? (double)p.weight[pair] : 1.0;
     if (threadIdx.x == 0) {
         // a side without weight adds nothing, also where it is infinite
@@ -760,6 +780,13 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
         o.rejected[pair] = (float)reward[1];
     }
     if (!o.grad) return;
+    if (falls) {
+        fill(0, T, __builtin_nanf(""));
+        return;
+    }
+    // tokens of no sequence: before the first, behind the last
+    fill(0, from < T ? from : T, 0.f);
+    fill(to < 0 ? 0 : to < T ? to : T, T, 0.f);
     // d loss / d u = sigma(u) - (1 - eps)
     const double slope = w == 0.0 && !bad ? 0.0 : w * (eps / (1.0 + exp(-u)) - (1.0 - eps) / (1.0 + exp(u)));
     const float g = (float)(q ? -slope * scale[1] : slope * scale[0]);
@@ -772,6 +799,17 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
         *reinterpret_cast<f32x4_any *>(o.grad + b + 4 * v) = d;
     }
     if (tail < e) o.grad[tail] = tail_on ? g : 0.f;
+}
+
+// Behind k_preference_loss: a workgroup that finds its part of the offsets to
+// descend writes NaN over everything (all that do write the same).
+__global__ __launch_bounds__(1024) void k_preference_order(dlr_preference p, PairOut o, int64_t part) {
+    const int64_t from = blockIdx.x * part, to = from + part < 2 * p.pairs ? from + part : 2 * p.pairs;
+    if (!__syncthreads_or(descend<1024>(p.offsets, from, to))) return;
+    const float nan = __builtin_nanf("");
+    for (int64_t i = threadIdx.x; i < p.pairs; i += 1024) o.loss[i] = o.chosen[i] = o.rejected[i] = nan;
+    if (!o.grad) return;
+    for (int64_t i = threadIdx.x; i < p.tokens; i += 1024) o.grad[i] = nan;
 }
 
 // -------------------------------------------------- head log-probabilities
@@ -1546,17 +1584,30 @@ hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &all, const dlr_p
     });
 }
 
+// Up to here a workgroup looks through all offsets itself, beyond a second launch
+// does (pairs of 146 tokens, us a call: 2,048 pairs 11.9 against 13.7, 4,096 22.6
+// against 15.3; 11.9 and 12.7 without looking).
+constexpr int64_t kLookPairs = 2048;
+
 hipError_t launch_preference_loss(hipStream_t st, const dlr_preference &p, float *loss, float *chosen,
                                   float *rejected, float *grad) {
     const int64_t blocks = p.pairs ? p.pairs : 1;
     const PairOut o{loss, chosen, rejected, grad};
+    const bool look = p.pairs <= kLookPairs;
     // A large workgroup for long sequences, where there are CUs for it (us by
     // 256 / 512 / 1,024 threads: 16 pairs of 1,000 tokens 5.7 / 4.7 / 5.3, 1,024
     // of 1,465 11 / 12 / 19, 64 of 23,400 - / 30 / 23).
     const int64_t each = p.tokens / blocks;
-    if (each > 8192) return launch(k_preference_loss<1024>, blocks, 1024, st, p, o);
-    if (each > 512 && blocks <= 2 * kCus) return launch(k_preference_loss<512>, blocks, 512, st, p, o);
-    return launch(k_preference_loss<256>, blocks, 256, st, p, o);
+    hipError_t e;
+    if (each > 8192)
+        e = launch(k_preference_loss<1024>, blocks, 1024, st, p, o, look);
+    else if (each > 512 && blocks <= 2 * kCus)
+        e = launch(k_preference_loss<512>, blocks, 512, st, p, o, look);
+    else
+        e = launch(k_preference_loss<256>, blocks, 256, st, p, o, look);
+    if (e != hipSuccess || look) return e;
+    const int64_t parts = (2 * p.pairs + 8191) / 8192 < 64 ? (2 * p.pairs + 8191) / 8192 : 64;
+    return launch(k_preference_order, parts, 1024, st, p, o, (2 * p.pairs + parts - 1) / parts);
 }
 
 // Whether the rows can go through the DMA kernels: 16-byte chunks of rows that

@@ -131,8 +131,9 @@ int dlr_policy_loss(int device, void *stream, const dlr_logits *x, const dlr_pol
  *   loss[p]  = -(1 - label_smoothing) log sigma(u) - label_smoothing log sigma(-u)
  * The objective is sum_p weight[p] * loss[p]; grad is its gradient with
  * respect to logprob: tokens without mask and tokens of no sequence get 0,
- * whatever their log-probabilities hold.  Offsets that are no ranges of the
- * tokens give NaN for their pair and its tokens. */
+ * whatever their log-probabilities hold.  A sequence that leaves the tokens
+ * gives NaN for its pair and its pair's tokens; offsets that descend anywhere
+ * (sequences would overlap) give NaN for every pair and token. */
 typedef struct dlr_preference {
     const float *logprob;       /* tokens                                     */
     const float *ref_logprob;   /* tokens; NULL: 0                            */
