@@ -388,6 +388,17 @@ __device__ inline void residual_row(const T *row, T *out, int vocab, int64_t y, 
 // with the type's lowest value) take their statistics again.
 constexpr float kLseExact = 128.f;
 
+// What 2^((z - m) k) is multiplied by to give exp(z / tau - l): 1 / s where the l
+// given is the row's own lse as far as 32 bits show (another rounding of it
+// included), less where it is of more classes than these, as a caller has it
+// who holds only some of them.
+__device__ inline double share_of_lse(BlockStat a, double tau, float l) {
+    if (a.s == 0.0 && l != NEG_INF) return 0.0;  // these classes have probability 0, others may not
+    const double own = a.m / tau + log(a.s), off = own - (double)l;
+    if ((float)own == l || fabs(off) <= 0x1p-23 * fabs(own)) return 1.0 / a.s;
+    return exp(off) / a.s;
+}
+
 // One row a workgroup, one read and one write.  Bound by memory: 4,096 x
 // 131,072 bf16 379 us (5.7 TB/s), 2,048 x 50,257 f16 with odd rows 71 us (5.1).
 template <typename T, int NT>
@@ -410,7 +421,7 @@ __global__ __launch_bounds__(NT) void k_token_logprob_grad(const T *logits, int6
     if (fabsf(l) > kLseExact) {
         __shared__ BlockLds<NT> lds;
         const BlockStat a = join_block<NT>(row_stat<T, NT, 4>(row, vocab, k, false), k, lds);
-        const float neg = (float)(-c / a.s), m = a.m;
+        const float neg = (float)(-c * share_of_lse(a, tau, l)), m = a.s == 0.0 && l != NEG_INF ? 0.f : a.m;
         residual_row<T, NT, 4>(row + begin, o, here, y - begin, c,
                                [=](float z) { return neg * exp2_scaled(z - m, k); }, once);
         return;

@@ -207,9 +207,9 @@ def token_logprob(logits: torch.Tensor, target: torch.Tensor, *,
 def token_logprob_grad(logits: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor, *,
                        temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient with respect to the logits of sum(grad * logprob), in the
-    logits' type; lse is token_logprob's.  Rows with a negative target or
-    grad 0 are 0.  out may be the logits themselves
-    (dlr_token_logprob_grad)."""
+    logits' type; lse is token_logprob's, or that of more classes than these.
+    Rows with a negative target or grad 0 are 0.  out may be the logits
+    themselves (dlr_token_logprob_grad)."""
     gpu, target, x = _logits(logits, target, temperature)
     lse = _vector("lse", lse, gpu, _F32, x.rows)
     grad = _vector("grad", grad, gpu, _F32, x.rows)

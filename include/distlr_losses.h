@@ -92,10 +92,12 @@ int dlr_token_logprob(int device, void *stream, const dlr_logits *x, void *works
 /* The gradient of sum_t grad[t] * logprob[t] with respect to the logits (the
  * softmax residual): grad_logits[t][j] = grad[t] / temperature * (1[j = y] -
  * exp(z_tj / temperature - lse[t])), in the logits' type, rows
- * grad_row_stride (>= vocab) elements apart.  lse is dlr_token_logprob's.  A
- * row with grad[t] = 0 is 0 whatever its logits hold.  grad_logits may be
- * x->data itself with the same stride (the logits are then overwritten);
- * any other overlap is refused. */
+ * grad_row_stride (>= vocab) elements apart.  lse is dlr_token_logprob's, or of
+ * more classes than these (of which target[t] is one).  32 bits are coarse for
+ * an lse beyond +-128: one that is the row's own up to its last bit is taken
+ * again from the row, any other as it is given.  A row with grad[t] = 0 is 0
+ * whatever its logits hold.  grad_logits may be x->data itself with the same
+ * stride (the logits are then overwritten); any other overlap is refused. */
 int dlr_token_logprob_grad(int device, void *stream, const dlr_logits *x, const float *lse, const float *grad,
                            void *grad_logits, int64_t grad_row_stride);
 
