@@ -1588,10 +1588,11 @@ hipError_t launch_policy_loss(hipStream_t st, const dlr_logits &all, const dlr_p
         if constexpr (sizeof(T) == 2) {
             if (packs <= 17 * 512) return launch_policy<T, 512, 16, 1>(st, x, p, po, out, out_stride);
             return launch_policy<T, 512, 8, 9, true>(st, x, p, po, out, out_stride);
+        } else {
+            if (packs <= 8192) return launch_policy<T, 512, 16>(st, x, p, po, out, out_stride);
+            if (packs <= 16384) return launch_policy<T, 1024, 16>(st, x, p, po, out, out_stride);
+            return launch_policy<T, 1024, 16, 0, true>(st, x, p, po, out, out_stride);
         }
-        if (packs <= 8192) return launch_policy<T, 512, 16>(st, x, p, po, out, out_stride);
-        if (packs <= 16384) return launch_policy<T, 1024, 16>(st, x, p, po, out, out_stride);
-        return launch_policy<T, 1024, 16, 0, true>(st, x, p, po, out, out_stride);
     });
 }
 
