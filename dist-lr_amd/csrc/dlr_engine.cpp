@@ -3539,6 +3539,7 @@ int dlr_load_train_dense(dlr_ctx *c, const dlr_dense *ds, int64_t batch_size, in
     if (int rc_ = wait_stream(c, c->stream, __func__)) return rc_;
     if (c->xstream)  // the pieced all-gather's stream carries collectives too
         if (int rc_ = wait_stream(c, c->xstream, __func__)) return rc_;
+    const int fault = c->fault;
     free_train(c);
     free_touched_bufs(c);
     int rc;
@@ -3590,11 +3591,20 @@ int dlr_load_train_dense(dlr_ctx *c, const dlr_dense *ds, int64_t batch_size, in
     if (stream) {
         t.streamed = true;
         t.hX = ds->X.data();
-        hipError_t e = hipHostRegister(const_cast<float *>(t.hX), xbytes, hipHostRegisterDefault);
-        // refused (or registered already): the rows are copied as they are,
-        // through the driver's own staging where they are pageable
+        hipError_t e = fault == dlr::kFaultLockRefused  ? hipErrorInvalidValue
+                       : fault == dlr::kFaultLockFailed ? hipErrorOutOfMemory
+                                                        : hipHostRegister(const_cast<float *>(t.hX), xbytes,
+                                                                          hipHostRegisterDefault);
         t.host_registered = e == hipSuccess;
         if (e != hipSuccess) (void)hipGetLastError();
+        // a driver that does not lock existing memory says 'invalid value' for
+        // every array; then (or where the caller has locked the rows) they are
+        // copied as they are, through the driver's own staging if pageable
+        if (e != hipSuccess && e != hipErrorInvalidValue && e != hipErrorNotSupported &&
+            e != hipErrorHostMemoryAlreadyRegistered) {
+            t.streamed = false;
+            return fail(c, DLR_E_HIP, std::string("dlr_load_train_dense: hipHostRegister: ") + hipGetErrorString(e));
+        }
         if (!c->cstream) HIPC(c, hipStreamCreateWithFlags(&c->cstream, hipStreamNonBlocking));
         for (int k = 0; k < 2; ++k) {
             if (!c->ev_ready[k]) HIPC(c, hipEventCreateWithFlags(&c->ev_ready[k], hipEventDisableTiming));
@@ -4001,7 +4011,7 @@ int dlr_stage_counters(dlr_ctx *c, int64_t *out, int n) {
 }
 
 int dlr_set_fault(dlr_ctx *c, int fault) {
-    if (!c || fault < dlr::kFaultNone || fault > dlr::kFaultHotRing)
+    if (!c || fault < dlr::kFaultNone || fault > dlr::kFaultLockFailed)
         return fail(c, DLR_E_ARG, "dlr_set_fault: bad fault");
     c->fault = fault;
     return DLR_OK;
@@ -4090,6 +4100,12 @@ int dlr_train_residency(dlr_ctx *c) {
     if (!c) return DLR_E_ARG;
     if (!c->train.loaded) return fail(c, DLR_E_STATE, "dlr_train_residency: no training shard loaded");
     return c->train.streamed || c->train.sparse_stream ? DLR_RESIDENCY_STREAM : DLR_RESIDENCY_DEVICE;
+}
+
+int dlr_train_host_locked(dlr_ctx *c) {
+    if (!c) return DLR_E_ARG;
+    if (!c->train.loaded) return fail(c, DLR_E_STATE, "dlr_train_host_locked: no training shard loaded");
+    return c->train.host_registered || c->train.sparse_stream ? 1 : 0;
 }
 
 int dlr_train_relabeled(dlr_ctx *c) {

@@ -143,7 +143,10 @@ enum DevFault {
     kFaultNone = 0,
     kFaultMgPublish = 1,   // k_grad_lds MG: margin block 0 never adds to its counter
     kFaultRefPublish = 2,  // k_dense_ref: margin unit 0 never adds to its slot's counter
-    kFaultHotRing = 3      // k_band_hot / k_hot_chain: the product / loader waves never post a chunk
+    kFaultHotRing = 3,     // k_band_hot / k_hot_chain: the product / loader waves never post a chunk
+    // the next dense load's page-locking of the caller's rows (not a kernel's)
+    kFaultLockRefused = 4,  // as by a driver that does not lock existing memory
+    kFaultLockFailed = 5    // out of memory
 };
 
 // The largest grid of `threads`-thread workgroups with `lds` bytes of

@@ -33,6 +33,7 @@ E_ARG = -1  # bad argument / shape mismatch
 E_DEVICE = -8  # an in-launch hand-off never came (dlr_sync)
 # test-only producer faults (dlr_set_fault)
 FAULT_NONE, FAULT_MG_PUBLISH, FAULT_REF_PUBLISH, FAULT_HOT_RING = 0, 1, 2, 3
+FAULT_LOCK_REFUSED, FAULT_LOCK_FAILED = 4, 5
 # dlr_stage_counters indices
 COUNT_HOT_CHAIN_LAUNCHES, COUNT_HOT_GIVEUPS, COUNT_COWAIT_SERIALISED, COUNT_MG_DEMOTED = 0, 1, 2, 3
 COUNTERS = 4
@@ -51,7 +52,7 @@ SYMBOLS = [
     "dlr_exchange_plan", "dlr_merge_range", "dlr_merge_touched", "dlr_rccl_trace",
     "dlr_get_unique_id", "dlr_create", "dlr_create_group", "dlr_comm_abort", "dlr_comm_info", "dlr_destroy", "dlr_last_error",
     "dlr_set_weights", "dlr_get_weights", "dlr_load_train", "dlr_load_test", "dlr_load_train_dense",
-    "dlr_load_test_dense", "dlr_set_residency", "dlr_train_residency",
+    "dlr_load_test_dense", "dlr_set_residency", "dlr_train_residency", "dlr_train_host_locked",
     "dlr_tuning_default", "dlr_tuning_from_env", "dlr_set_tuning", "dlr_get_tuning", "dlr_set_summation_order",
     "dlr_summation_order",
     "dlr_train_step", "dlr_train_epoch", "dlr_worker_gradient", "dlr_server_apply", "dlr_predict", "dlr_sync",
@@ -169,6 +170,7 @@ _sig("dlr_load_train_dense", C.c_int, P, P, i64, C.POINTER(i64))
 _sig("dlr_load_test_dense", C.c_int, P, P)
 _sig("dlr_set_residency", C.c_int, P, C.c_int)
 _sig("dlr_train_residency", C.c_int, P)
+_sig("dlr_train_host_locked", C.c_int, P)
 _sig("dlr_set_summation_order", C.c_int, P, C.c_int)
 _sig("dlr_summation_order", C.c_int, P)
 _sig("dlr_dataset_write_libsvm", C.c_int, P, C.c_char_p, C.c_int)
@@ -618,6 +620,14 @@ class Engine:
         self._c(min(rc, 0))
         return rc
 
+    def train_host_locked(self) -> bool:
+        """Whether the loaded shard's host copy is page-locked: False for a
+        streamed dense shard means slower, pageable copies
+        (dlr_train_host_locked)."""
+        rc = lib.dlr_train_host_locked(self._h)
+        self._c(min(rc, 0))
+        return bool(rc)
+
     def set_summation_order(self, order: int) -> None:
         """ORDER_REFERENCE (default: every sum in lr.cc's order, bitwise the
         reference's arithmetic) or ORDER_FAST (deterministic reordered long
@@ -661,7 +671,8 @@ class Engine:
 
     def set_fault(self, fault: int) -> None:
         """TEST ONLY: withhold one in-launch producer (FAULT_*) in the next
-        steps; they must then raise DLRError(E_DEVICE) (dlr_set_fault)."""
+        steps; they must then raise DLRError(E_DEVICE).  FAULT_LOCK_*: the next
+        streamed dense load's page-locking (dlr_set_fault)."""
         self._c(lib.dlr_set_fault(self._h, fault))
 
     def timing(self, enable: bool) -> None:

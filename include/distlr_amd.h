@@ -301,12 +301,19 @@ int dlr_load_test_dense(dlr_ctx *ctx, const dlr_dense *ds);
  * layout except band mode, whose one >= 2^21-row batch is not worth
  * streaming: DLR_E_ARG).  AUTO (default) streams only when the shard would
  * not leave 8 GiB of HBM free.  Results are bitwise identical either way.
- * dlr_train_residency reports what the loaded shard uses. */
+ * dlr_train_residency reports what the loaded shard uses;
+ * dlr_train_host_locked 1 if its host copy is page-locked: 0 for a streamed
+ * dense shard means that each batch's copy goes through the driver's staging,
+ * slower, and may hold the calling thread (also where the caller had locked the
+ * rows before, whose copies are fast).  A page-locking that fails for another
+ * reason than that existing memory cannot be locked fails the load
+ * (DLR_E_HIP). */
 #define DLR_RESIDENCY_AUTO 0
 #define DLR_RESIDENCY_DEVICE 1
 #define DLR_RESIDENCY_STREAM 2
 int dlr_set_residency(dlr_ctx *ctx, int mode);
 int dlr_train_residency(dlr_ctx *ctx);
+int dlr_train_host_locked(dlr_ctx *ctx);
 
 /* TUNING of the loads (one struct instead of scattered switches).  The
  * engine picks layouts and kernel forms itself at dlr_load_train* time;
@@ -438,7 +445,9 @@ int dlr_sync(dlr_ctx *ctx);
 /* TEST ONLY: withhold one producer of the next steps' in-launch hand-offs
  * (0 = none; 1 = the one-launch step's margin block 0 never publishes; 2 =
  * K6r's margin unit 0 never publishes; 3 = k_band_hot's product waves never
- * post) -- the steps must then fail with DLR_E_DEVICE. */
+ * post) -- the steps must then fail with DLR_E_DEVICE.  Or the page-locking of
+ * the next streamed dense load: 4 = refused (the rows stay pageable), 5 = out of
+ * memory (the load fails). */
 int dlr_set_fault(dlr_ctx *ctx, int fault);
 
 /* Per-kernel timing with HIP events on the context's stream.  enable=1
