@@ -30,6 +30,7 @@ STAGE_MARGIN, STAGE_GRADIENT, STAGE_UPDATE = 0, 1, 2
 TRANSPORT_NONE, TRANSPORT_RCCL, TRANSPORT_LOOPBACK = 0, 1, 2
 ORDER_REFERENCE, ORDER_FAST = 0, 1
 E_ARG = -1  # bad argument / shape mismatch
+E_HIP = -4  # a HIP call failed
 E_DEVICE = -8  # an in-launch hand-off never came (dlr_sync)
 # test-only producer faults (dlr_set_fault)
 FAULT_NONE, FAULT_MG_PUBLISH, FAULT_REF_PUBLISH, FAULT_HOT_RING = 0, 1, 2, 3
@@ -241,6 +242,35 @@ def _check(rc: int, ctx=None):
         msg = lib.dlr_last_error(ctx)
         raise DLRError(rc, msg.decode(errors="replace") if msg else "")
     return rc
+
+
+def hip_runtimes() -> List[str]:
+    """The HIP runtimes this process has loaded.  More than one: torch's and
+    ROCm's, because this package came before torch; only the one that is used
+    first sees the GPU."""
+    try:
+        with open("/proc/self/maps") as f:
+            paths = {line.split(maxsplit=5)[-1].strip() for line in f if "/libamdhip64.so" in line}
+    except OSError:
+        return []
+    return sorted(paths)
+
+
+def _two_runtimes() -> str:
+    found = hip_runtimes()
+    return "" if len(found) < 2 else (f" (this process has {len(found)} HIP runtimes, of which one sees the GPU: "
+                                      f"{', '.join(found)}; import torch before distlr_amd)")
+
+
+def _created(rc: int) -> None:
+    """A context's creation; no GPU found has one more cause than the library knows."""
+    try:
+        _check(rc)
+    except DLRError as e:
+        why = _two_runtimes() if e.code == E_HIP else ""
+        if not why:
+            raise
+        raise DLRError(e.code, lib.dlr_last_error(None).decode(errors="replace") + why) from None
 
 
 def _ptr(a: Optional[np.ndarray]):
@@ -547,7 +577,7 @@ class Engine:
         if _handle is None:
             h = P()
             uid = C.create_string_buffer(unique_id, UNIQUE_ID_BYTES) if unique_id is not None else None
-            _check(lib.dlr_create(device, rank, world, uid, num_feature_dim, C.byref(h)))
+            _created(lib.dlr_create(device, rank, world, uid, num_feature_dim, C.byref(h)))
             _handle = h
         self._h = _handle
         self.n_batches = 0
@@ -559,7 +589,7 @@ class Engine:
         RCCL.  Drive each engine from its own thread (collectives block until
         every rank arrives)."""
         hs = (P * world)()
-        _check(lib.dlr_create_group(device, world, num_feature_dim, hs))
+        _created(lib.dlr_create_group(device, world, num_feature_dim, hs))
         return [cls(num_feature_dim, device, r, world, _handle=P(hs[r])) for r in range(world)]
 
     def comm_abort(self, why: str = "aborted") -> None:

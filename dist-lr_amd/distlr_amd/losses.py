@@ -22,7 +22,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import E_ARG, PKG, DLRError
+from . import E_ARG, PKG, DLRError, _two_runtimes
 
 LIB_PATH = os.path.join(PKG, "lib", "libdistlr_losses.so")
 LIB_PATH = os.environ.get("DLR_LOSSES_LIB", LIB_PATH)  # as DLR_LIB: a variant build of the same library
@@ -112,7 +112,7 @@ def _gpu(name: str, t) -> int:
     if not isinstance(t, torch.Tensor):
         _refuse(f"{name} must be a torch tensor")
     if not t.is_cuda:
-        _refuse(f"{name} must be on a GPU (it is on {t.device})")
+        _refuse(f"{name} must be on a GPU (it is on {t.device})" + ("" if torch.cuda.is_available() else _two_runtimes()))
     return t.get_device()
 
 
