@@ -58,6 +58,16 @@ bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
     return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
 }
 
+// Rows of `cols` bytes, `a_stride` and `b_stride` bytes apart.  Rows at the same
+// distance may lie between each other's.
+bool rows_overlap(const void *a, int64_t a_stride, const void *b, int64_t b_stride, int64_t rows, int64_t cols) {
+    if (!overlap(a, (rows - 1) * a_stride + cols, b, (rows - 1) * b_stride + cols)) return false;
+    if (rows == 1 || a_stride != b_stride || a_stride == 0) return true;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const int64_t apart = (int64_t)((x < y ? y - x : x - y) % (uintptr_t)a_stride);
+    return apart < cols || a_stride - apart < cols;
+}
+
 constexpr int64_t kMaxRows = INT64_C(0x7fffffff);
 constexpr int64_t kMaxPairs = (INT64_C(1) << 22) - 1;  // one launch of at most 1,024 threads each
 constexpr int64_t kMaxVocab = INT64_C(1) << 30;
@@ -95,8 +105,7 @@ const char *check_grad(const dlr_logits *x, const void *grad, int64_t stride) {
     if (stride < 0 || !spans(x->rows, x->vocab, stride, 4)) return "grad_row_stride is out of range";
     const int64_t b = element_bytes(x->dtype);
     const bool same = grad == x->data && (stride == x->row_stride || x->rows == 1);
-    if (!same && overlap(x->data, ((x->rows - 1) * x->row_stride + x->vocab) * b, grad,
-                         ((x->rows - 1) * stride + x->vocab) * b))
+    if (!same && rows_overlap(x->data, x->row_stride * b, grad, stride * b, x->rows, x->vocab * b))
         return "grad_logits overlaps the logits and is not the logits themselves";
     if (same && x->rows > 1 && x->row_stride == 0) return "grad_logits cannot be logits whose rows share memory";
     return nullptr;

@@ -97,7 +97,8 @@ int dlr_token_logprob(int device, void *stream, const dlr_logits *x, void *works
  * an lse beyond +-128: one that is the row's own up to its last bit is taken
  * again from the row, any other as it is given.  A row with grad[t] = 0 is 0
  * whatever its logits hold.  grad_logits may be x->data itself with the same
- * stride (the logits are then overwritten); any other overlap is refused. */
+ * stride (the logits are then overwritten); any other overlap is refused (rows
+ * between the logits' rows, at the same stride, are none). */
 int dlr_token_logprob_grad(int device, void *stream, const dlr_logits *x, const float *lse, const float *grad,
                            void *grad_logits, int64_t grad_row_stride);
 
