@@ -167,9 +167,13 @@ def _grad_like(logits: torch.Tensor, out: Optional[torch.Tensor], gpu: int) -> t
     _matrix("out", out, gpu)
     if out.dtype != logits.dtype or out.shape != logits.shape:
         _refuse("out must have the logits' type and shape")
-    if not out.is_inference():
-        torch.autograd.graph.increment_version(out)  # autograd sees that a tensor it may have saved is written
     return out
+
+
+def _written(out: Optional[torch.Tensor]) -> None:
+    """Autograd sees that a tensor of the caller's, which it may have saved, was written."""
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)
 
 
 def _rows(out: torch.Tensor):
@@ -213,10 +217,11 @@ def token_logprob_grad(logits: torch.Tensor, target: torch.Tensor, lse: torch.Te
     gpu, target, x = _logits(logits, target, temperature)
     lse = _vector("lse", lse, gpu, _F32, x.rows)
     grad = _vector("grad", grad, gpu, _F32, x.rows)
-    out = _grad_like(logits, out, gpu)
+    dz = _grad_like(logits, out, gpu)
     _check(lib.dlr_token_logprob_grad(gpu, _stream(gpu), C.byref(x), lse.data_ptr(), grad.data_ptr(),
-                                      out.data_ptr(), out.stride(0)))
-    return out
+                                      dz.data_ptr(), dz.stride(0)))
+    _written(out)
+    return dz
 
 
 def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logprob: torch.Tensor, advantage: torch.Tensor, *,
@@ -251,6 +256,7 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logprob: torch.T
     need, scratch = _scratch(x, logits)
     _check(lib.dlr_policy_loss(gpu, _stream(gpu), C.byref(x), C.byref(p), _ptr(scratch), need, at, at + 4 * rows,
                                at + 8 * rows, clipped.data_ptr(), _ptr(dz), 0 if dz is None else dz.stride(0)))
+    _written(out)
     return PolicyLoss(loss, logprob, kl, clipped, dz)
 
 

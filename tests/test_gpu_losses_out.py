@@ -27,3 +27,20 @@ def test_a_gradient_beside_the_logits(L, dtype, rows, vocab):  # noqa: F811
     got = L.policy_loss(z, y, lp, g, weight=g, out=out)
     assert torch.equal(out, want.grad) and torch.equal(got.loss, want.loss)
     assert torch.equal(z, keep) and torch.equal(both[:, 2 * vocab:], rest)
+
+
+def test_a_refused_call_leaves_the_tensors_version(L, dlr):  # noqa: F811
+    z = torch.randn(6, 40, device="cuda")
+    y, v = make_target(4, 40).cuda(), torch.zeros(4, device="cuda")
+    calls = [lambda out, **kw: L.token_logprob_grad(z[:4], y, v, v, out=out, **kw),
+             lambda out, **kw: L.policy_loss(z[:4], y, v, v, out=out, **kw)]
+    for call in calls:
+        for bad, kw in ((z[1:5], {}), (torch.empty(4, 40, device="cuda"), dict(temperature=0.0))):
+            before = bad._version
+            with pytest.raises(dlr.DLRError):
+                call(bad, **kw)
+            assert bad._version == before
+        out = torch.empty(4, 40, device="cuda")
+        before = out._version
+        call(out)
+        assert out._version == before + 1
