@@ -72,3 +72,53 @@ def test_logprob_gradient_errs_to_no_side(L, rows, vocab, shift, temperature):  
     # and at most half a step of 256: 2^-17
     bound = 3 * U + EXP + 50 * U / math.sqrt(vocab) + 2.0 ** -17 * 5 / math.sqrt(vocab) * (abs(shift) < 100)
     assert float(err.max()) <= bound, float(err.max())
+
+
+# Errors of lse, with rows shifted so that it is about 0 and its own rounding does
+# not hide them.  The sum's terms are off by random shares of U that average out,
+# and by the exponentials' mean; its roundings in a tree are random too.  So the mean
+# over the rows is within EXP + U, and one row's (a spread of a quarter of U and its
+# own rounding, U / 2 up to 1) within 2 U of that.
+def check_errors(lse, want):
+    err = lse.double() - want
+    assert float(want.abs().max()) <= 1.0
+    assert float(err.mean().abs()) <= EXP + U, float(err.mean())
+    assert float(err.pow(2).mean().sqrt()) <= EXP + 2 * U, float(err.pow(2).mean().sqrt())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("temperature", [0.7, 1.0, 1.3])
+@pytest.mark.parametrize("rows,vocab", [(400, 1000), (400, 50257), (300, 131072), (100, 131072)])
+def test_lse_errs_to_no_side(L, rows, vocab, temperature, dtype):  # noqa: F811
+    z = wide_logits(rows, vocab, 0.0, vocab)
+    z -= torch.logsumexp(z.double() / temperature, 1, keepdim=True).float() * temperature
+    if dtype == "bf16":
+        z = z.bfloat16()
+    want = torch.logsumexp(z.double() / temperature, 1)
+    y = torch.randint(0, vocab, (rows,), generator=gen(1)).cuda()
+    lp, lse = L.token_logprob(z, y, temperature=temperature)
+    check_errors(lse, want)
+    # logprob: the same lse, rounded where it is about 10
+    exact = z.double().gather(1, y[:, None])[:, 0] / temperature - want
+    err = lp.double() - exact
+    step = exact.abs() * U
+    assert bool((err.abs() <= step + EXP + 2 * U + 4 * U).all()), float(err.abs().max())
+
+
+@pytest.mark.parametrize("rows,vocab,dim", [(400, 50257, 520), (300, 20011, 264), (16, 131072, 520), (130, 9000, 261)])
+def test_head_lse_errs_to_no_side(L, rows, vocab, dim):  # noqa: F811
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim)
+    x = torch.randint(-2, 3, (rows, dim), generator=g, device="cuda").bfloat16()
+    w = torch.randint(-2, 3, (vocab, dim), generator=g, device="cuda").bfloat16()
+    scale = 0.8 * math.sqrt(dim)
+    # four columns of every class take each row's lse off: whole numbers up to 256 are exact
+    x[:, -4:], w[:, -4:] = 0.0, -1.0
+    z = torch.mm(x.double(), w.double().t())
+    off = torch.round(torch.logsumexp(z / scale, 1) * scale)
+    x[:, -4:] = torch.stack([torch.floor((off + i) / 4) for i in range(4)], 1).bfloat16()
+    z = torch.mm(x.double(), w.double().t())
+    assert float((z - torch.round(z)).abs().max()) == 0.0
+    y = torch.randint(0, vocab, (rows,), generator=gen(1)).cuda()
+    _, lse = L.head_logprob(x, w, y, temperature=scale)
+    check_errors(lse, torch.logsumexp(z / scale, 1))
