@@ -690,20 +690,21 @@ __device__ inline bool descend(const int64_t *offsets, int64_t from, int64_t to)
 // the pair's one slope written over its tokens.  4 tokens a thread and step,
 // loaded whether the mask counts them or not: a load that waits for its mask
 // costs a second trip to memory.  Bound by latency, three dependent trips and
-// the logarithms: 1,024 pairs of 1.5M tokens 11 us (19.6 a token at a time
+// the logarithms: 1,024 pairs of 1.5M tokens 13.5 us (19.6 a token at a time
 // behind its mask), two pairs 4.  One workgroup a pair also where the
-// sequences are very long (1 x 400,000 tokens 69 us): the logits of such a
+// sequences are very long (1 x 400,000 tokens 55 us): the logits of such a
 // pair take a thousand times as long.
 //
 // Offsets that descend anywhere make sequences overlap, and which workgroup
 // would write a shared token's gradient last is nobody's to say: then every pair
-// and token is NaN.  `look`: each workgroup looks through the offsets for itself;
-// else k_preference_order does, behind this launch.
+// and token is NaN.  `look`: each workgroup looks through the offsets for itself (1
+// of the 13.5 us); else k_preference_order does, behind this launch.
 template <int NT>
 __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOut o, bool look) {
     constexpr int H = NT / 2, W = NT / 64;
     __shared__ double sums[W];
     __shared__ int64_t counts[W];
+    __shared__ int descends[W];
     const int64_t P = p.pairs, T = p.tokens;
     // tokens [b, e) of the gradient, by all workgroups
     auto fill = [&](int64_t b, int64_t e, float v) {
@@ -714,8 +715,6 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
         return;
     }
     const int64_t from = p.offsets[0], to = p.offsets[2 * P];
-    bool falls = false;
-    if (look) falls = descend<NT>(p.offsets, 0, 2 * P);
     const int64_t pair = blockIdx.x;
     const int q = threadIdx.x / H, at = threadIdx.x % H;
     int64_t first[2], last[2];
@@ -733,6 +732,7 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     const int64_t b = q ? first[1] : first[0], e = q ? last[1] : last[0];
     auto mask4 = [&](int64_t i) { return p.mask ? *reinterpret_cast<const u32_any *>(p.mask + i) : 0x01010101u; };
     const int64_t packs = (e - b) / 4, tail = b + packs * 4 + at;
+    const bool wave_falls = look && __any(descend<NT>(p.offsets, 0, 2 * P));
     double sum = 0.0;
     int64_t count = 0;
 #pragma unroll 4
@@ -762,11 +762,12 @@ __global__ __launch_bounds__(NT) void k_preference_loss(dlr_preference p, PairOu
     if ((threadIdx.x & 63) == 0) {
         sums[threadIdx.x >> 6] = sum;
         counts[threadIdx.x >> 6] = count;
+        descends[threadIdx.x >> 6] = wave_falls;
     }
-    if (look)
-        falls = __syncthreads_or(falls);
-    else
-        __syncthreads();
+    __syncthreads();
+    bool falls = false;
+#pragma unroll
+    for (int w = 0; w < W; ++w) falls |= descends[w] != 0;
     double reward[2], scale[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
