@@ -280,7 +280,10 @@ __global__ __launch_bounds__(NT) void k_token_logprob(const T *logits, int64_t s
 // A CU alone reads a long row slowly.  Up to 128 rows of 8,192 packs and more
 // go by chunks: their statistics to scratch memory (and the target's logit,
 // which the gradient may then overwrite), a second launch joins them.  1 x
-// 131,072 bf16: 5.9 us, 10.9 by one workgroup; the policy loss 8.6, 18.8.
+// 131,072 bf16: 5.9 us, 10.9 by one workgroup; the policy loss 8.6, 18.8.  From
+// about 160 rows on a workgroup a row is as fast (129 rows, logprob and policy
+// loss: 13.5 and 28.5 by chunks, 14.1 and 29.5 by rows; 160: 14.2 and 31.9, 15.0
+// and 30.8; 255: 18.3 and 43.1, 16.6 and 36.9).
 struct RowPart {
     double s;
     float m;
@@ -862,6 +865,9 @@ constexpr int kTileV = 128, kTileT = 128, kTileK = 64, kLdsRow = kTileK + 8;
 // MFMA in 32 bits, never written; per token the tile's (maximum, sum) goes
 // to part[tile][token], and the target's logit to zy[token].  Classes lie
 // along the MFMA's rows, so a token's values sit in one lane column.
+// For rows that the DMA cannot take.  Bound by its stages, fetched through
+// registers between two barriers with nothing to multiply meanwhile: 333 x 1535
+// x 50257 bf16 200 us, 68 at dim 1536 by DMA; 1 x 4095 x 131072 475, 180.
 template <typename T>
 __global__ __launch_bounds__(256) void k_head_tile(dlr_head h, float2 *part, float *zy) {
     __shared__ __attribute__((aligned(16))) uint16_t sw[kTileV * kLdsRow];
@@ -984,9 +990,12 @@ __global__ __launch_bounds__(1024) void k_head_pick(const void *target, int targ
 #define SCHED_LDS(n) __builtin_amdgcn_sched_group_barrier(256, n, 0)
 
 // Measured (bf16): 256 x 256 tiles, 8 waves of 128 x 64, 4096 x 4096 x 65536
-// 1.57 ms, 1,400 TFLOP/s, softmax included, where the library's product alone
-// takes 1.54; the matrix cores are busy 75% of the cycles, at the 1.8 GHz that
-// they leave of the clock.  4 waves of 128 x 128 read a third less from LDS, but
+// 1.57 to 1.60 ms once the clock has settled (the first ten launches after a pause
+// up to 2.1), 1,380 TFLOP/s, softmax included, where the library's product alone
+// takes 1.46 to 1.54; the matrix cores are busy 72 to 75% of the cycles, at the 1.8
+// GHz that they leave of the clock.  A tile's ends (filling the stages, the softmax,
+// nothing else on the CU) are 9 to 10 us beside 1.4 a stage: 4096 x 512 x 131072 676
+// us, 813 TFLOP/s.  4 waves of 128 x 128 read a third less from LDS, but
 // the compiler then moves accumulators between register files (994 TFLOP/s);
 // 32 x 32 products meet LDS banks twice in this layout (1,109); a workgroup
 // that goes on to its next tile and fetches it under this one's end spills
@@ -1647,7 +1656,8 @@ static HeadSpace head_space(void *workspace, int64_t rows) {
 }
 
 // Whether the rows that take part are picked first, so that the others cost
-// nothing: 4 us for what may be half of a long call, from about 100 us on.
+// nothing: 3 to 5 us at 277 rows, 7 at 4,096, for what may be half of a long
+// call, from about 100 us on.
 static bool head_picks(const dlr_head &h) {
     return (double)h.rows * (double)h.vocab * (double)h.dim >= 6.4e10 && h.rows > 64;
 }
@@ -1676,7 +1686,9 @@ static hipError_t launch_head_waves(hipStream_t st, dlr_head h, int64_t first, i
 
 // The tiles of more than 16 rows.  What a tile costs: microseconds per stage
 // of 64, alone on its CU or two of them on it, measured from 1 x 8 to 32,768
-// tiles at dim 512 and 4096; and per round of the CUs its ends.
+// tiles at dim 512 and 4096; and per round of the CUs a part of its ends (a fit
+// for choosing between tiles: a 256 x 256 tile is 1.4 a stage and ends of 9 to 10,
+// so that short dimensions cost more than this says, by any tile).
 struct HeadTile {
     int64_t tv, tt;
     double alone, two;  // two 0: one workgroup a CU
