@@ -91,3 +91,27 @@ def test_ascending_offsets_outside_the_tokens(L):  # noqa: F811
         out = L.preference_loss(lp, None, torch.tensor(offsets).cuda(), beta=0.1)
         for g, kind in zip(out.grad.tolist(), kinds):
             assert {"n": g != g, "0": g == 0, "g": 0 < abs(g) < 0.1}[kind], (offsets, out.grad)
+
+
+@pytest.mark.parametrize("pairs", [5, 3000])
+def test_captured_offsets_change_between_replays(L, pairs):  # noqa: F811
+    # ascending, descending and ascending offsets through one graph, with eager work in between
+    tokens = 3 * pairs + 40
+    lp = torch.randn(tokens, generator=gen(10)).cuda()
+    offsets = packed(pairs, tokens, 11).cuda()
+    L.preference_loss(lp, None, offsets, beta=0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = L.preference_loss(lp, None, offsets, beta=0.1)
+    for seed in range(6):
+        new = packed(pairs, tokens, 20 + seed, seed % 3, seed % 2)
+        if seed % 2:
+            new[pairs] = tokens + 1 - new[pairs - 1]  # another place
+            new[pairs + 1] = new[pairs] - 1
+        offsets.copy_(new)
+        want = [t.clone() for t in L.preference_loss(lp, None, offsets, beta=0.1)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(out, want)), seed
+        assert all_nan(out) == bool(seed % 2)
