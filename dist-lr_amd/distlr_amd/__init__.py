@@ -270,7 +270,7 @@ def _created(rc: int) -> None:
         why = _two_runtimes() if e.code == E_HIP else ""
         if not why:
             raise
-        raise DLRError(e.code, lib.dlr_last_error(None).decode(errors="replace") + why) from None
+        raise DLRError(e.code, (lib.dlr_last_error(None) or b"").decode(errors="replace") + why) from None
 
 
 def _ptr(a: Optional[np.ndarray]):
