@@ -623,8 +623,8 @@ struct HeldRow {
 // statistics, so the row stays on the CU until they are known.  REST: rows
 // longer than (R + Q) NT packs; what does not fit is read again, from the
 // Infinity Cache.
-// Bound by memory: 4,096 x 131,072 bf16 415 us (5.2 TB/s; reading all of the
-// row a second time instead of holding it 547), 1,021 x 50,257 f32 85 us.  The
+// Bound by memory: 4,096 x 131,072 bf16 419 us (5.1 TB/s; reading all of the
+// row a second time instead of holding it 547), 1,021 x 50,257 f32 86 us.  The
 // exponentials of a row's two passes take two thirds of its time, so another
 // row has to be on the CU beside it.  Loading the next row into the registers
 // that the gradient frees spilled them (882 us).
